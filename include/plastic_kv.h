@@ -59,6 +59,7 @@ extern "C" {
 #define PI_DTYPE_F32 0
 #define PI_DTYPE_BF16 1
 #define PI_DTYPE_F16 2
+#define PI_DTYPE_E4M3 3 /* pools of the 8-bit cache only (pi_rope_append, pi_*_q8) */
 
 /* Version of this ABI (bumped on any signature change). */
 int pi_abi_version(void);
@@ -434,6 +435,43 @@ int pi_decode_prologue(void* q_out, int64_t q_out_stride, void* k_pool, void* v_
                        const int64_t* positions, const int64_t* slot_mapping, int batch,
                        int num_q_heads, int num_kv_heads, int head_dim, int page_size,
                        int64_t num_slots, int pool_dtype, int* err, cudaStream_t stream);
+
+/*
+ * Rotary append of any number of tokens (prompts and decode steps; no single reference
+ * counterpart: qk_norm, rope_positions and _write_kv_layer of the reference runners,
+ * src/plastic_infer/exec/attention.py:23-95, src/plastic_infer/exec/runner_paged.py:112-129,
+ * with the rotary forms they lack). For each token t at position positions[t]:
+ *   q_out[t, h]  = rope(qknorm(q_in[t, h], q_norm_w), positions[t])      h < Hq
+ *   K slot[t], h = rope(qknorm(k_in[t, h], k_norm_w), positions[t])      h < Hkv
+ *   V slot[t], h = v_in[t, h]
+ * qknorm as in pi_decode_prologue (skipped when both weights are NULL). rope turns the first
+ * 2 * rot_pairs elements of a head and leaves the others; pair j is (j, j + rot_pairs), or
+ * (2j, 2j + 1) with `interleaved`, the angle positions[t] * inv_freq[j] is formed in 64 bits,
+ * and rope_scale multiplies cosine and sine (the attention factor of stretched contexts; 1
+ * otherwise). fp32 arithmetic, one rounding to the output type. slot_mapping[t] < 0 writes no
+ * K/V row for t; a slot past the pool is skipped and reported through `err`.
+ *   q_in, k_in, v_in   `in_dtype`, heads contiguous, token strides in elements
+ *   q_out              the pools' type, or in_dtype with 8-bit pools
+ *   pools              physical [num_pages, Hkv, page_size, head_dim], `pool_dtype`
+ *
+ * pool_dtype PI_DTYPE_E4M3: K and V are kept as e4m3 values times one scale per (page, KV
+ * head), k_scale / v_scale fp32 [num_pages, Hkv] (NULL for the other types). Tokens of a call
+ * with consecutive slots inside a page form a run. The run's block gets the scale 2^e,
+ *   e = max(e of the kept rows, the smallest e >= -118 with amax <= 448 * 2^e),
+ * amax over the run's finite values; kept rows are those at offsets below the run's first
+ * (a run at offset 0 keeps none and starts the block anew), rescaled when e grows. Values
+ * beyond +-448 * 2^e (infinities) saturate, NaN stays NaN, rows behind the run are left as
+ * they were. At most one run per page and call: with several, or with a slot named twice,
+ * which of their rows and scales a page ends up with is unspecified (nothing else is touched).
+ */
+int pi_rope_append(void* q_out, int64_t q_out_stride, void* k_pool, void* v_pool, float* k_scale,
+                   float* v_scale, const void* q_in, int64_t q_in_stride, const void* k_in,
+                   int64_t k_in_stride, const void* v_in, int64_t v_in_stride, int in_dtype,
+                   const void* q_norm_w, const void* k_norm_w, float eps, const float* inv_freq,
+                   int rot_pairs, int interleaved, float rope_scale, const int64_t* positions,
+                   const int64_t* slot_mapping, int64_t n_tokens, int num_q_heads,
+                   int num_kv_heads, int head_dim, int page_size, int64_t num_pages,
+                   int pool_dtype, int* err, cudaStream_t stream);
 
 /*
  * Contiguous gather of a request's pages in the reference's gather layout:

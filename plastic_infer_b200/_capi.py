@@ -37,6 +37,7 @@ PI_ATTN_RING_SHALLOW = 2
 PI_DTYPE_F32 = 0
 PI_DTYPE_BF16 = 1
 PI_DTYPE_F16 = 2
+PI_DTYPE_E4M3 = 3  # pools of the 8-bit cache only
 
 ABI_VERSION = 3
 
@@ -105,6 +106,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _f32, _vp, _vp, _vp,
          _i32, _i32, _i32, _i32, _i32, _i64, _i32, _vp, _vp],
+    ),
+    # q_out, q_out_stride, k_pool, v_pool, k_scale, v_scale, q_in, q_in_stride, k_in,
+    # k_in_stride, v_in, v_in_stride, in_dtype, q_norm_w, k_norm_w, eps, inv_freq, rot_pairs,
+    # interleaved, rope_scale, positions, slot_mapping, n_tokens, hq, hkv, head_dim, page_size,
+    # num_pages, pool_dtype, err, stream
+    "pi_rope_append": (
+        _i32,
+        [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _f32,
+         _vp, _i32, _i32, _f32, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _vp, _vp],
     ),
     # q_len, num_q_heads, num_kv_heads, head_dim, kv_len
     "pi_host_stream_attn_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i64]),

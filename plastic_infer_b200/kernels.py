@@ -16,6 +16,10 @@ These are the batched additions behind the reference's single-request API:
                          per-rank outputs fused in (NVLink peer stores; multi-GPU)
   decode_prologue        QK-norm + RoPE of a step's q/k rows and the K/V slot write, one
                          launch (reference: attention.py:23-95 + _write_kv_layer)
+  rope_append            QK-norm + rotary positions (half or interleaved pairs, part of the head,
+                         scaled) of any number of tokens and their K/V slot write, one launch;
+                         16/32-bit pools, or e4m3 pools with a scale per (page, KV head)
+  rope_frequencies       rotary frequencies for rope_append: plain, or scaled for long contexts
   paged_prefill_attention
                          one request's prefill straight from the pool
                          (reference: _attn_paged, src/plastic_infer/exec/runner_paged.py:36-95)
@@ -222,6 +226,192 @@ def decode_prologue(
         qw.data_ptr() if qw is not None else None, kw.data_ptr() if kw is not None else None,
         float(eps), inv_freq.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(),
         B, Hq, Hkv, D, S, P * S, dtype_code(k_pool.dtype), _err_ptr(err), _stream(),
+    )
+    return q_out
+
+
+# ---------------------------------------------------------------------------
+# Rotary append (any number of tokens; 16/32-bit or 8-bit pools)
+# ---------------------------------------------------------------------------
+
+ROPE_SCALINGS = ("none", "linear", "ntk", "yarn")
+
+
+def rope_frequencies(rotary_dim: int, base: float, scaling: str = "none", factor: float = 1.0,
+                     trained_len: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                     device: torch.device | str = "cpu") -> tuple[torch.Tensor, float]:
+    """(inv_freq fp32 [rotary_dim / 2], rope_scale) for rope_append.
+
+    "none"    1 / base^(2j / rotary_dim), rope_scale 1
+    "linear"  every frequency divided by `factor` (positions interpolated)
+    "ntk"     base raised to base * factor^(R / (R - 2)): the slowest pair is stretched by
+              `factor`, the fastest not at all
+    "yarn"    pairs that turn fewer than beta_slow times in the trained length are divided by
+              `factor`, those that turn more than beta_fast times are kept, a linear ramp over
+              the pair index in between; rope_scale = 0.1 ln(factor) + 1
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be positive and even, got {rotary_dim}")
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"scaling must be one of {ROPE_SCALINGS}, got {scaling!r}")
+    if scaling != "none" and not factor >= 1.0:
+        raise ValueError("factor must be at least 1")
+    if scaling == "ntk":
+        if rotary_dim <= 2:
+            raise ValueError("ntk scaling needs rotary_dim > 2")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    inv = 1.0 / base ** (torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    rope_scale = 1.0
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "yarn":
+        if trained_len <= 0:
+            raise ValueError("yarn scaling needs trained_len")
+
+        def pair_turning(turns: float) -> float:  # index of the pair with that many turns
+            return (rotary_dim * math.log(trained_len / (turns * 2 * math.pi))
+                    / (2 * math.log(base)))
+
+        low = max(math.floor(pair_turning(beta_fast)), 0)
+        high = min(math.ceil(pair_turning(beta_slow)), rotary_dim // 2 - 1)
+        ramp = (torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)
+        keep = 1.0 - ramp.clamp(0, 1)
+        inv = inv / factor * (1 - keep) + inv * keep
+        rope_scale = 0.1 * math.log(factor) + 1.0
+    return inv.float().to(device), rope_scale
+
+
+def _check_scales(k_scale: torch.Tensor | None, v_scale: torch.Tensor | None, pages: int,
+                  heads: int) -> None:
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if t is None or t.dtype != torch.float32 or tuple(t.shape) != (pages, heads) \
+                or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 [{pages}, {heads}] tensor: one "
+                             "scale per (page, KV head) of an 8-bit pool")
+
+
+def _check_one_device(*tensors: torch.Tensor | None) -> torch.device:
+    """The one CUDA device that every given tensor is on."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _require_cuda(t)
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"all tensors must be on one device, got {device} and {t.device}")
+    return device  # type: ignore[return-value]
+
+
+def _call_on(device: torch.device, func: str, *args) -> None:
+    """_capi.call on the current stream of `device`, with that device current."""
+    if device.index == torch.cuda.current_device():
+        _capi.call(func, *args, torch.cuda.current_stream(device).cuda_stream)
+        return
+    with torch.cuda.device(device):
+        _capi.call(func, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def rope_append(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    q_norm_weight: torch.Tensor | None = None,
+    k_norm_weight: torch.Tensor | None = None,
+    eps: float = 1e-5,
+    interleaved: bool = False,
+    rope_scale: float = 1.0,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+    q_out: torch.Tensor | None = None,
+    err: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """QK-norm (optional) and rotary positions of T new q and k rows, and the write of the new
+    K/V rows at their slots; one launch for a decode step or for whole prompts.
+
+    q [T, Hq, D], k / v [T, Hkv, D]: heads contiguous, any token strides (e.g. slices of a
+    fused QKV output). positions int64 [T]; slot_mapping int64 [T] (page * page_size + offset;
+    < 0: no K/V row). inv_freq fp32 [R / 2] turns the first R elements of a head
+    (rope_frequencies): pairs (j, j + R/2), or (2j, 2j + 1) with `interleaved`; rope_scale
+    multiplies cosine and sine. Angles are formed in 64 bits, so far positions keep their
+    precision. Returns q_out [T, Hq, D].
+
+    16/32-bit pools take the rows in the pool dtype, which is q_out's too. Pools of
+    torch.float8_e4m3fn need k_scale and v_scale, fp32 [num_pages, Hkv] (q_out then has q's
+    dtype): each (page, head) block has one power-of-two scale, grown as rows arrive; the rows
+    of one call in one page must be consecutive tokens with consecutive slots, rows at lower
+    offsets are kept (rescaled when the scale grows), rows behind are left as they were
+    (include/plastic_kv.h has the formulas).
+    """
+    P, Hkv, S, D = _check_pool(k_pool, "k_pool")
+    if v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype:
+        raise ValueError("k_pool and v_pool must have the same shape and dtype")
+    if not v_pool.is_contiguous():
+        raise ValueError("v_pool must be contiguous")
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"q must be [T, Hq, {D}], got {tuple(q.shape)}")
+    T, Hq = q.shape[0], q.shape[1]
+    if tuple(k.shape) != (T, Hkv, D) or k.shape != v.shape:
+        raise ValueError(f"k and v must be [{T}, {Hkv}, {D}]")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError("q, k and v must share one dtype")
+    in_code = dtype_code(q.dtype)
+    eight = k_pool.dtype == torch.float8_e4m3fn
+    if eight:
+        _check_scales(k_scale, v_scale, P, Hkv)
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError("k_scale and v_scale go with pools of torch.float8_e4m3fn")
+    pool_code = _capi.PI_DTYPE_E4M3 if eight else dtype_code(k_pool.dtype)
+    out_dtype = q.dtype if eight else k_pool.dtype
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.stride(2) != 1 or t.stride(1) != D:
+            raise ValueError(f"{name}: heads must be contiguous rows of head_dim elements")
+    if positions.dtype != torch.int64 or positions.shape != (T,):
+        raise ValueError("positions must be int64 [T]")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (T,):
+        raise ValueError("slot_mapping must be int64 [T]")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > D:
+        raise ValueError(f"inv_freq must be float32 [R / 2] with R <= {D}")
+    if (q_norm_weight is None) != (k_norm_weight is None):
+        raise ValueError("give both QK-norm weights or neither")
+    if q_out is None:
+        q_out = torch.empty((T, Hq, D), dtype=out_dtype, device=q.device)
+    elif q_out.dtype != out_dtype or tuple(q_out.shape) != (T, Hq, D) or q_out.stride(2) != 1 \
+            or q_out.stride(1) != D:
+        raise ValueError(f"q_out must be [T, Hq, D] {out_dtype} with contiguous heads")
+    qw = kw = None
+    if q_norm_weight is not None:
+        qw = q_norm_weight.to(q.dtype).contiguous()
+        kw = k_norm_weight.to(q.dtype).contiguous()
+        if qw.numel() != D or kw.numel() != D:
+            raise ValueError(f"QK-norm weights must have {D} elements")
+    device = _check_one_device(q, k, v, positions, inv_freq, slot_mapping, k_pool, v_pool, q_out,
+                               qw, kw, k_scale, v_scale, err)
+    if T == 0:
+        return q_out
+    positions = positions.contiguous()
+    slot_mapping = slot_mapping.contiguous()
+    inv_freq = inv_freq.contiguous()
+    # (one token: its stride is never used, and torch may report any)
+    row, kv_row = Hq * D, Hkv * D
+    strides = (q_out.stride(0), q.stride(0), k.stride(0), v.stride(0)) if T > 1 \
+        else (row, row, kv_row, kv_row)
+    _call_on(
+        device, "pi_rope_append",
+        q_out.data_ptr(), strides[0], k_pool.data_ptr(), v_pool.data_ptr(),
+        k_scale.data_ptr() if eight else None, v_scale.data_ptr() if eight else None,
+        q.data_ptr(), strides[1], k.data_ptr(), strides[2], v.data_ptr(), strides[3], in_code,
+        qw.data_ptr() if qw is not None else None, kw.data_ptr() if kw is not None else None,
+        float(eps), inv_freq.data_ptr(), inv_freq.shape[0], 1 if interleaved else 0,
+        float(rope_scale), positions.data_ptr(), slot_mapping.data_ptr(), T, Hq, Hkv, D, S, P,
+        pool_code, _err_ptr(err),
     )
     return q_out
 
