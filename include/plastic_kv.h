@@ -474,6 +474,39 @@ int pi_rope_append(void* q_out, int64_t q_out_stride, void* k_pool, void* v_pool
                    int pool_dtype, int* err, cudaStream_t stream);
 
 /*
+ * Batched paged GQA decode attention over an 8-bit cache (no reference counterpart: the
+ * reference keeps its cache in the model's type). As pi_paged_decode_attn, with pools of e4m3
+ * values and one fp32 scale per (page, KV head), k_scale / v_scale [num_pages, num_kv_heads]
+ * (as pi_rope_append leaves them; any finite scale >= 0 is read):
+ *   out[b, hq, :] = softmax(scale * q[b, hq, :] . (sk K)_b[hq / G]^T) (sv V)_b[hq / G]
+ * over the first min(ctx_lens[b], max_pages * page_size) tokens of request b; none: zeros.
+ * What lies behind a request's last token, in its last page or elsewhere, is not used,
+ * whatever bytes it holds. fp32 softmax and accumulation; q and the softmax weights enter the
+ * products as sums of e4m3 parts, two for bf16 and three for f16.
+ *
+ *   q, out         [batch, num_q_heads, head_dim] of `dtype` (f32, bf16, f16), request strides
+ *   block_tables   [batch, max_pages] int32, rows bt_stride elements apart (0: one table for all)
+ *   workspace      pi_paged_decode_attn_q8_workspace_bytes(head_dim) bytes, 256-byte aligned,
+ *                  whose first pi_paged_decode_attn_q8_ws_zero_bytes() are zero before the first
+ *                  call; every call leaves them zero (after PI_ERR_TIMEOUT in `err`, zero them
+ *                  again). Calls that share one must be ordered. NULL is accepted where
+ *                  the generic kernel runs: f32, head sizes other than 64, 128 and 256, pages
+ *                  other than 16 and 32.
+ * head_dim <= 256. A page id outside the pool is reported through `err`, and the outputs of
+ * that request are then unspecified.
+ */
+size_t pi_paged_decode_attn_q8_workspace_bytes(int head_dim);
+size_t pi_paged_decode_attn_q8_ws_zero_bytes(void);
+int pi_paged_decode_attn_q8(void* out, const void* q, const void* k_pool, const void* v_pool,
+                            const float* k_scale, const float* v_scale,
+                            const int32_t* block_tables, int64_t bt_stride, int max_pages,
+                            const int32_t* ctx_lens, int batch, int num_q_heads,
+                            int num_kv_heads, int head_dim, int page_size, int64_t num_pages,
+                            float scale, int dtype, int64_t q_stride, int64_t out_stride,
+                            void* workspace, size_t workspace_bytes, int* err,
+                            cudaStream_t stream);
+
+/*
  * Contiguous gather of a request's pages in the reference's gather layout:
  *   out[t, h, :] = pool[block_table[t / page_size], h, t % page_size, :]
  * for t in [0, num_tokens). out is [num_tokens, kv_heads, head_dim].

@@ -116,6 +116,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _f32,
          _vp, _i32, _i32, _f32, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _vp, _vp],
     ),
+    "pi_paged_decode_attn_q8_workspace_bytes": (_sz, [_i32]),
+    "pi_paged_decode_attn_q8_ws_zero_bytes": (_sz, []),
+    # out, q, k_pool, v_pool, k_scale, v_scale, block_tables, bt_stride, max_pages, ctx_lens,
+    # batch, hq, hkv, head_dim, page_size, num_pages, scale, dtype, q_stride, out_stride,
+    # workspace, workspace_bytes, err, stream
+    "pi_paged_decode_attn_q8": (
+        _i32,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i64,
+         _f32, _i32, _i64, _i64, _vp, _sz, _vp, _vp],
+    ),
     # q_len, num_q_heads, num_kv_heads, head_dim, kv_len
     "pi_host_stream_attn_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i64]),
     # out, q, q_tok_stride, out_tok_stride, spans (host array), num_spans, q_len, q_start,

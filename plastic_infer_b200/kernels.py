@@ -20,6 +20,8 @@ These are the batched additions behind the reference's single-request API:
                          scaled) of any number of tokens and their K/V slot write, one launch;
                          16/32-bit pools, or e4m3 pools with a scale per (page, KV head)
   rope_frequencies       rotary frequencies for rope_append: plain, or scaled for long contexts
+  paged_decode_attention_q8
+                         decode attention over e4m3 pools with a scale per (page, KV head)
   paged_prefill_attention
                          one request's prefill straight from the pool
                          (reference: _attn_paged, src/plastic_infer/exec/runner_paged.py:36-95)
@@ -629,6 +631,112 @@ def paged_decode_attention(
         block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(),
         B, Hq, Hkv, D, S, P, float(scale), dtype_code(q.dtype), q.stride(0), out.stride(0),
         ws.data_ptr(), ws.numel(), _err_ptr(err), _stream(),
+    )
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Attention over an 8-bit cache
+# ---------------------------------------------------------------------------
+
+_q8_ws: dict[tuple[int, int], Workspace] = {}
+_q8_ws_bytes: dict[tuple[int, int], int] = {}
+
+
+def _check_q8_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor) -> tuple[int, int, int, int]:
+    P, Hkv, S, D = _check_pool(k_pool, "k_pool")
+    if k_pool.dtype != torch.float8_e4m3fn or v_pool.dtype != torch.float8_e4m3fn:
+        raise TypeError("the pools must be torch.float8_e4m3fn")
+    if v_pool.shape != k_pool.shape or not v_pool.is_contiguous():
+        raise ValueError("v_pool must be contiguous and have k_pool's shape")
+    _check_scales(k_scale, v_scale, P, Hkv)
+    return P, Hkv, S, D
+
+
+def _q8_workspace(device: torch.device, head_dim: int, workspace: Workspace | None) -> torch.Tensor:
+    """Scratch for one q8 attention call on the device's current stream: the caller's, or one
+    of the stream's own, so that calls on two streams never share it. Under graph capture it
+    comes out of the graph's memory, zeroed by the graph: no two graphs share it either."""
+    key = (device.index, head_dim)
+    nbytes = _q8_ws_bytes.get(key)
+    if nbytes is None:
+        with torch.cuda.device(device):
+            nbytes = int(_capi.load().pi_paged_decode_attn_q8_workspace_bytes(head_dim))
+        _q8_ws_bytes[key] = nbytes
+    if workspace is not None:
+        if torch.device(workspace.device).index not in (None, device.index):
+            raise ValueError(f"the workspace is on {workspace.device}, q on {device}")
+        return workspace.get(nbytes)
+    if torch.cuda.is_current_stream_capturing():
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf[:int(_capi.load().pi_paged_decode_attn_q8_ws_zero_bytes())].zero_()
+        return buf
+    stream = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    ws = _q8_ws.get(stream)
+    if ws is None:
+        with _ws_lock:
+            ws = _q8_ws.setdefault(stream, Workspace(device))
+    return ws.get(nbytes)
+
+
+def paged_decode_attention_q8(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_tables: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+    workspace: Workspace | None = None,
+    err: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Decode attention of q [B, Hq, D] over each request's first ctx_lens[b] tokens of an
+    8-bit cache: pools torch.float8_e4m3fn [num_pages, Hkv, page_size, D] with fp32 scales
+    [num_pages, Hkv], as rope_append fills them.
+
+    block_tables int32 [B, max_pages], ctx_lens int32 [B]. Returns out [B, Hq, D] in q's dtype
+    (bf16, f16 or f32); a request with no context gets zeros. What lies behind a request's last
+    token is not used, whatever it holds. Head sizes 64, 128 and 256 with pages of 16 or 32 run
+    on the tensor cores in bf16 and f16; everything else (head_dim <= 256) on a plain kernel.
+    Without `workspace`, calls on different streams and captured graphs have scratch of their own.
+    """
+    P, Hkv, S, D = _check_q8_pools(k_pool, v_pool, k_scale, v_scale)
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"q must be [B, Hq, {D}], got {tuple(q.shape)}")
+    B, Hq, _ = q.shape
+    if Hq == 0 or Hq % Hkv != 0:
+        raise ValueError(f"num_q_heads {Hq} not a multiple of num_kv_heads {Hkv}")
+    code = dtype_code(q.dtype)
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != B:
+        raise ValueError("block_tables must be int32 [B, max_pages]")
+    if ctx_lens.dtype != torch.int32 or ctx_lens.shape != (B,):
+        raise ValueError("ctx_lens must be int32 [B]")
+    device = _check_one_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, ctx_lens, out, err)
+    if q.stride(2) != 1 or q.stride(1) != D or (B > 1 and q.stride(0) < Hq * D):
+        q = q.contiguous()
+    if block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    ctx_lens = ctx_lens.contiguous()
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=device)
+    elif out.shape != (B, Hq, D) or out.dtype != q.dtype or out.stride(2) != 1 or out.stride(1) != D:
+        raise ValueError("out must be [B, Hq, D] with contiguous heads, q's dtype")
+    if B == 0:
+        return out
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    ws = _q8_workspace(device, D, workspace)
+    row = Hq * D
+    _call_on(
+        device, "pi_paged_decode_attn_q8",
+        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), block_tables.data_ptr(), block_tables.stride(0) if B > 1 else 0,
+        block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv, D, S, P, float(scale), code,
+        q.stride(0) if B > 1 else row, out.stride(0) if B > 1 else row, ws.data_ptr(), ws.numel(),
+        _err_ptr(err),
     )
     return out
 
