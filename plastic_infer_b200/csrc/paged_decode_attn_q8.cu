@@ -3,37 +3,41 @@
 //
 //   out[b, hq] = sum_t p_t sv(t) V[t] / sum_t p_t,   p_t = exp(scale * sk(t) q . K[t] - max)
 //
-// What bounds it: K and V once, HBM. At half the bytes of a 16-bit cache the arithmetic per
-// byte doubles, so the values are never widened: both products run on the tensor cores in e4m3
-// (mma.sync m16n8k32, which measured 0.90 per clock and SM here against 0.48 for the 16-bit
-// m16n8k16), and the 16-bit operands are split into e4m3 parts whose sum they are:
-//   q 2^k = q1 + q2 (+ q3),  each part the e4m3 rounding of what the ones before leave.
-// A bf16 value has 8 significant bits and two parts hold it exactly (down to 2^-18 of the row's
-// largest element); an f16 value has 11 and takes three. P is split the same way (two parts:
-// 2^-8 relative, as near as bf16; three for f16: 2^-12). The parts ride in the n dimension: up to
-// four query heads per KV head, part 1 is columns 0-3 and part 2 columns 4-7 of one MMA.
+// What bounds it: K and V once, HBM. At half the bytes of a 16-bit cache the arithmetic per byte
+// doubles, and mma.sync has no 8-bit float form of its own on sm_100a: m16n8k32 e4m3 measured 0.13
+// per clock and SM with fresh operands, against 0.30 for the 16-bit m16n8k16 it is put together
+// from. So a unit's values are widened once, in registers, by cvt.rn.f16x2.e4m3x2 (1.2 per clock
+// and SM; every e4m3 value is an f16 value), and both products are f16 MMAs with fp32 sums:
+//   q 2^k in f16: exact for bf16 (down to 2^-22 of the row's largest element, which k brings into
+//   [128, 256)) and for f16;
+//   P in f16, relative to the unit's own maximum and to its larger V scale, times 256: 2^-12 of
+//   each weight, down to 2^-32 of the unit's largest.
 //
 // A step of a warp is a unit of 32 tokens (two pages of 16, or one of 32):
-//   S^T[tokens, cols] = K[tokens, D] . Q^T            A = K by ldmatrix, rows of 32 bytes
+//   S^T[tokens, heads] = K[tokens, D] . Q^T           A = K by ldmatrix, widened
 //   softmax of the unit against its own maximum, then
-//   O^T[D, cols] = alpha O^T + beta (V^T[D, tokens] . P^T[tokens, cols])
-//                                                     A = V^T by ldmatrix .b8 transposed
-// P is relative to the unit's maximum and to its larger V scale, times 256: e4m3's range covers
-// every unit alike, whatever the running maximum, and what P loses below 2^-18 of the unit's
-// largest weight stays below 2^-18 of that unit's share. beta = 2^(max_unit - max) sv.
-// The S^T accumulator becomes the P^T operand with one movmatrix per 16 tokens: a 16-bit element
-// carries the bytes of two tokens, and the token order that leaves is made good by the row
-// addresses of V's ldmatrix. The MMA rows 8..15 are tokens 12..15, 8..11, which keeps both K's
-// and V's ldmatrix free of bank conflicts in the 128-byte swizzle.
+//   O^T[D, heads] = alpha O^T + beta (V^T[D, tokens] . P^T[tokens, heads])
+//                                                     A = V^T by ldmatrix .b8 transposed, widened
+// beta = 2^(max_unit - max) sv. A lane's four bytes of K or V become the two k pairs of a fragment;
+// the order of the elements along k that this implies is put into Q's loads, and for V into the
+// row addresses of its ldmatrix. The MMA rows 8..15 are tokens 12..15, 8..11, which keeps both
+// K's and V's ldmatrix free of bank conflicts in the 128-byte swizzle.
 //
 // Work: the stream of units over (request, KV head) is cut into equal ranges, one per resident
 // warp, each with its own ring of TMA stages; pieces of a cut (request, head) are merged by the
 // last warp to finish one (the counters return to zero). More than eight query heads per KV
 // head run as several passes over it.
 //
+// Measured on B200 (32 query and 8 KV heads of 128): 64 requests of 512-8192 tokens, 572 MB, in
+// 103 us, 5.5 TB/s, 0.84 of the measured copy rate; 8 of 32k (f16, pages of 32) in 96 us, 0.82; 128 of
+// 200-4096 with 8 query heads per KV head, 286 MB, in 62 us, 0.70. What is left: some 4 us until the
+// first loads are out, and the spread of the warps' ends (the same SMs are up to 15 % late in every
+// launch). One CTA per SM with loader warps, items from a queue and a quarter of the stream handed
+// out dynamically evened the ends out, but its waits for items and partial sums cost more than
+// that: 129 us for the first.
+//
 // Generic kernel (fp32 queries, other head sizes and pages): one CTA per (request, query head).
 #include <atomic>
-#include <type_traits>
 
 #include <cuda_fp8.h>
 #include <cudaTypedefs.h>
@@ -47,7 +51,7 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode();  // paged_decode_attn.cu
 
 namespace q8 {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;  // per CTA, each an independent consumer
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 32;            // tokens per step
 constexpr int kMaxBatch = 4096;
@@ -82,25 +86,65 @@ template <int D>
 struct Cfg {
   static constexpr int kTile = kUnit * D;      // bytes of K (or V) of a unit
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kKK = D / 32;           // k steps of Q K^T
+  static constexpr int kKK = D / 16;           // k steps of Q K^T
   static constexpr int kDT = D / 16;           // m tiles of V^T P^T
-  // Two CTAs per SM with three stages at D = 128 keep 192 KB of loads in flight per SM.
-  static constexpr int kStages = D == 64 ? 5 : 3;
+  // 128 KB of loads in flight per SM (two CTAs; one at D = 256). More only lengthens the queue in
+  // front of HBM, where every small access waits too, and pulls the SMs apart: with three stages
+  // at D = 128 (192 KB) 64 requests of 512-8192 tokens took 114 us against 105, 8 of 32k 104
+  // against 96.
+  static constexpr int kStages = D == 64 ? 4 : 2;
+  static_assert(kWarps * kStages % 2 == 0, "the stages' scales follow their barriers, 16-byte aligned");
 };
 
 template <int D>
 constexpr size_t smem_bytes(int batch) {
   return 1024 + static_cast<size_t>(kWarps) * Cfg<D>::kStages * (Cfg<D>::kStage + 8 + 16) +
-         static_cast<size_t>(batch + 1) * 4;
+         static_cast<size_t>(2 * batch + 1) * 4;
 }
 
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+// (not volatile: pure functions of their operands, free to be scheduled)
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
       " {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                             uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+      " {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Four e4m3 values as two f16 pairs (exact).
+__device__ __forceinline__ void widen(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(v));
+}
+
+// Paired fp32 multiply and fused multiply-add.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 // Two 16 x 16 byte matrices, transposed: lane l receives bytes (rows 4 (l % 4) .. + 3) of columns
@@ -113,22 +157,9 @@ __device__ __forceinline__ void ldmatrix_b8_trans_x2(uint32_t addr, uint32_t& r0
                : "r"(addr));
 }
 
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-}
-
-__device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
-  return __half22float2(
-      __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v), __NV_E4M3)));
-}
-
-// Nearest value with four significant bits (ties away from zero): what e4m3 keeps of x.
-__device__ __forceinline__ float round4(float x) {
-  return __uint_as_float((__float_as_uint(x) + 0x00080000u) & 0xfff00000u);
-}
-
-// Byte offset o of a tile (rows of 128 bytes, 1024-byte aligned) in the 128-byte swizzle.
-__device__ __forceinline__ uint32_t sw(uint32_t o) { return o ^ (((o >> 7) & 7u) << 4); }
+// Byte offset o of a tile (rows of 128 bytes, 1024-byte aligned) in the 128-byte swizzle. Linear
+// over xor, so sw(lane's part) ^ sw(constant) addresses the sum of two disjoint offsets.
+__host__ __device__ constexpr uint32_t sw(uint32_t o) { return o ^ (((o >> 7) & 7u) << 4); }
 
 // Token of a unit's 16-token half behind MMA row r.
 __device__ __forceinline__ int row_token(int r) { return r < 8 ? r : 8 + ((r - 8) ^ 4); }
@@ -137,53 +168,92 @@ __device__ __forceinline__ int clamp_ctx(int ctx, int max_tokens) {
   return min(max(ctx, 0), max_tokens);
 }
 
-// out = sum_j w_j O_j / sum_j w_j l_j over a segment's pieces, w_j = 2^(m_j - max m).
+// out = sum_j w_j O_j / sum_j w_j l_j over the np pieces of a segment, w_j = 2^(m_j - max m). One
+// warp, often at the launch's end, so latency counts: all heads at once in float4 columns, several
+// pieces' loads in flight before any is used.
 template <typename T, int D>
 __device__ __noinline__ void merge_pieces(T* dst, const float* ws_ml, const float* ws_o, int wa,
-                                          int npieces, int role_a, int heads, int lane) {
+                                          int np, int role_a, int heads, int lane) {
   auto slot_of = [&](int j) { return static_cast<int64_t>(wa + j) * 2 + (j == 0 ? role_a : 0); };
-  for (int g = 0; g < heads; ++g) {
-    float M = -INFINITY;
-    for (int j = lane; j < npieces; j += 32)
-      M = fmaxf(M, __ldcg(ws_ml + (slot_of(j) * kHeadsPad + g) * 2));
+  constexpr int E = kHeadsPad * D / 128;  // float4 columns per lane, all heads
+  constexpr int kPerHead = D / 4;
+  constexpr int kCols = E < 4 ? E : 4;    // columns at a time
+  constexpr int kPieces = 4;              // pieces at a time
+  const int n4 = heads * kPerHead;
+  const int hd = min(lane & 7, heads - 1);
+  const float2* mls = reinterpret_cast<const float2*>(ws_ml) + hd;
+  // maximum and sum of head lane % 8, pieces lane / 8 of every four
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int j = lane >> 3; j < np; j += 4) top = fmaxf(top, __ldcg(mls + slot_of(j) * kHeadsPad).x);
+  top = fmaxf(top, __shfl_xor_sync(kFull, top, 8));
+  top = fmaxf(top, __shfl_xor_sync(kFull, top, 16));
+  for (int e0 = 0; 32 * e0 < n4; e0 += kCols) {
+    float4 acc[kCols];
+    float sum[kCols], tops[kCols];
 #pragma unroll
-    for (int x = 16; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor_sync(kFull, M, x));
-    float L = 0.f;
-    float acc[D / 32];
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
-#pragma unroll 8
-    for (int j = 0; j < npieces; ++j) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws_ml + (slot_of(j) * kHeadsPad + g) * 2));
-      const float w = ml.x == M ? 1.f : fast_exp2(ml.x - M);
-      L += w * ml.y;
-      const float* src = ws_o + (slot_of(j) * kHeadsPad + g) * D + lane * (D / 32);
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] += w * __ldcg(src + e);
+    for (int e = 0; e < kCols; ++e) {
+      acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      sum[e] = 0.f;
+      tops[e] = __shfl_sync(kFull, top, (min(lane + 32 * (e0 + e), n4 - 1) / kPerHead) & 7);
     }
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    for (int j0 = 0; j0 < np; j0 += kPieces) {
+      float4 v[kPieces][kCols];
+      float2 ml[kPieces][kCols];
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) dst[g * D + lane * (D / 32) + e] = from_f32<T>(acc[e] * inv);
+      for (int jj = 0; jj < kPieces; ++jj) {
+        const int64_t s = slot_of(min(j0 + jj, np - 1));
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) {  // (a branch here would put the loads one after another)
+          const int c = min(lane + 32 * (e0 + e), n4 - 1);
+          v[jj][e] = __ldcg(reinterpret_cast<const float4*>(ws_o + s * kHeadsPad * D) + c);
+          ml[jj][e] = __ldcg(reinterpret_cast<const float2*>(ws_ml) + s * kHeadsPad + c / kPerHead);
+        }
+      }
+#pragma unroll
+      for (int jj = 0; jj < kPieces; ++jj) {
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) {
+          float a = ml[jj][e].x == tops[e] ? 1.f : fast_exp2(ml[jj][e].x - tops[e]);
+          if (j0 + jj >= np) a = 0.f;
+          sum[e] += a * ml[jj][e].y;
+          acc[e].x += a * v[jj][e].x;
+          acc[e].y += a * v[jj][e].y;
+          acc[e].z += a * v[jj][e].z;
+          acc[e].w += a * v[jj][e].w;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) {
+      const int c = lane + 32 * (e0 + e);
+      if (c < n4) {
+        const float inv = 1.f / sum[e];
+        T* o = dst + 4 * c;
+        o[0] = from_f32<T>(acc[e].x * inv);
+        o[1] = from_f32<T>(acc[e].y * inv);
+        o[2] = from_f32<T>(acc[e].z * inv);
+        o[3] = from_f32<T>(acc[e].w * inv);
+      }
+    }
   }
 }
 
-// kWide: five to eight query heads of a pass, each part in an MMA of its own; else up to four.
-template <typename T, int D, int S, bool kWide>
+template <typename T, int D, int S>
 __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     decode_q8_kernel(const __grid_constant__ CUtensorMap tmap_k,
                      const __grid_constant__ CUtensorMap tmap_v, const Params p) {
   using C = Cfg<D>;
   constexpr int NS = C::kStages;
   constexpr int NP = kUnit / S;  // pages per unit
-  constexpr int kParts = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
-  constexpr int NT = kWide ? kParts : (kParts + 1) / 2;  // MMAs per step along n
   constexpr int kRows = S * D / 128;  // 128-byte rows per page tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kWarps * NS * C::kStage);
   float4* s_scale = reinterpret_cast<float4*>(bars + kWarps * NS);  // (sk0, sk1, sv0, sv1)
-  int* s_uoff = reinterpret_cast<int*>(s_scale + kWarps * NS);
+  int* s_uoff = reinterpret_cast<int*>(s_scale + kWarps * NS);  // first unit of each request
+  int* s_ctx = s_uoff + p.batch + 1;
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -198,9 +268,12 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     __shared__ int warp_tot[kWarps];
     const int per = (B + kThreads - 1) / kThreads;
     const int beg = min(tid * per, B), end = min(beg + per, B);
-    auto units = [&](int i) { return (clamp_ctx(__ldg(p.ctx_lens + i), max_tokens) + kUnit - 1) / kUnit; };
+    auto units = [&](int i) { return (s_ctx[i] + kUnit - 1) / kUnit; };
     int local = 0;
-    for (int i = beg; i < end; ++i) local += units(i);
+    for (int i = beg; i < end; ++i) {
+      s_ctx[i] = clamp_ctx(__ldg(p.ctx_lens + i), max_tokens);
+      local += units(i);
+    }
     int incl = local;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -231,23 +304,28 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
   const int NW = gridDim.x * kWarps;
   const int gw = blockIdx.x * kWarps + warp;
   const int64_t total = static_cast<int64_t>(s_uoff[B]) * HV;
-  // every active warp owns at least one unit: a segment's pieces are the warps that overlap it
-  const int NWe = static_cast<int>(total < NW ? total : NW);
+  // Every active warp owns at least one unit: a segment's pieces are the warps that overlap it. Two
+  // at least where there are enough: a piece more costs its merge more than a unit costs its warp
+  // (1000 tokens of 8 KV heads: 14.6 us against 16.5 with one unit per warp).
+  const int64_t most = (total + 1) / 2;
+  const int NWe = static_cast<int>(most < NW ? most : NW);
   const bool active = gw < NWe;
   const int64_t lo = active ? total * gw / NWe : 0;
   const int64_t hi = active ? total * (gw + 1) / NWe : 0;
 
-  auto locate = [&](int64_t pos, int& b, int& hv, int& u) {
+  // (request, head pass, unit) of a stream position; positions fit 32 bits (fast_shape)
+  auto locate = [&](int64_t pos64, int& b, int& hv, int& u) {
+    const int pos = static_cast<int>(pos64);
     int l = 0, r = B - 1;
     while (l < r) {
       const int mid = (l + r + 1) >> 1;
-      if (static_cast<int64_t>(s_uoff[mid]) * HV <= pos) l = mid; else r = mid - 1;
+      if (s_uoff[mid] * HV <= pos) l = mid; else r = mid - 1;
     }
     b = l;
     const int n = s_uoff[l + 1] - s_uoff[l];
-    const int64_t rem = pos - static_cast<int64_t>(s_uoff[l]) * HV;
-    hv = static_cast<int>(rem / n);
-    u = static_cast<int>(rem - static_cast<int64_t>(hv) * n);
+    const int rem = pos - s_uoff[l] * HV;
+    hv = rem / n;
+    u = rem - hv * n;
   };
 
   // Page tiles (page id * hkv + head) of stream position base + lane; -1: the unit has no second
@@ -262,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     int b, hv, u;
     locate(pos, b, hv, u);
     const int h = hv / p.passes;
-    const int n_pages = (clamp_ctx(__ldg(p.ctx_lens + b), max_tokens) + S - 1) / S;
+    const int n_pages = (s_ctx[b] + S - 1) / S;
     const int32_t* row = p.block_tables + static_cast<int64_t>(b) * p.bt_stride + u * NP;
     auto tile = [&](int i) {
       int pid = __ldg(row + i);
@@ -300,8 +378,6 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     }
   }
   if (!active) return;
-  sc_cur = load_scales(id_cur);
-  sc_nxt = load_scales(id_nxt);
 
   auto issue = [&](int64_t pos, int stage) {
     if (pos - pbase >= 32) {
@@ -314,7 +390,6 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     const int src = static_cast<int>(pos - pbase);
     const int t0 = __shfl_sync(kFull, id_cur.t0, src);
     const int t1 = __shfl_sync(kFull, id_cur.t1, src);
-    if (lane == src) my_scale[stage] = sc_cur;
     if (lane == 0) {
       const uint32_t bar = bar0 + 8 * stage;
       const uint32_t kdst = tiles_u32 + stage * C::kStage;
@@ -330,47 +405,47 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     }
   };
 
+  // the scales of the unit just issued, beside its stage
+  auto put_scales = [&](int64_t pos, int stage) {
+    if (lane == static_cast<int>(pos - pbase)) my_scale[stage] = sc_cur;
+  };
+
+  // the first loads go out before anything waits for the scales
   int64_t issued = lo;
   for (int s = 0; s < NS && issued < hi; ++s, ++issued) issue(issued, s);
+  sc_cur = load_scales(id_cur);
+  sc_nxt = load_scales(id_nxt);
+  for (int s = 0; s < issued - lo; ++s) put_scales(lo + s, s);
 
   const int gid = lane >> 2;
   const int tig = lane & 3;
   // K: matrix lane / 8, row lane % 8: rows 0-7 / 8-15, bytes 0-15 / 16-31 of each 32
   const int k_tok = row_token((lane & 7) + 8 * ((lane >> 3) & 1));
-  const uint32_t k_off = static_cast<uint32_t>(k_tok * D + 16 * (lane >> 4));
-  // V: row i = lane % 16 of matrix lane / 16 is the token of k slot i
+  const uint32_t k_sw = sw(static_cast<uint32_t>(k_tok * D + 16 * (lane >> 4)));
+  // V: row i = 4 t + j of a matrix is k slot 2 t + j (j < 2) or 8 + 2 t + j - 2
   const int vi = lane & 15;
-  const int v_tok = row_token(2 * (vi >> 2) + ((vi & 3) >> 1) + 8 * (vi & 1));
-  const uint32_t v_off = static_cast<uint32_t>((16 * (lane >> 4) + v_tok) * D);
+  const int v_tok = row_token(2 * (vi >> 2) + (vi & 1) + 8 * ((vi >> 1) & 1));
+  const uint32_t v_sw = sw(static_cast<uint32_t>((16 * (lane >> 4) + v_tok) * D));
   const int r0_tok = gid, r1_tok = 8 + (gid ^ 4);  // tokens of accumulator rows gid, gid + 8
-  const int head_a = kWide ? 2 * tig : (2 * tig) & 3;  // heads of accumulator columns
-  const bool first_part = tig < 2;
 
-  uint32_t qf[NT][C::kKK][2];
-  float f0, f1;  // 2^-k scale log2(e) of the two heads
-  // Query rows of (request b, head pass hv) as e4m3 parts; heads beyond the pass are zero.
+  uint32_t qf[C::kKK][2];
+  float f0, f1;  // 2^-k scale log2(e) of heads 2 tig and 2 tig + 1
+  // Query rows of (request b, head pass hv) in f16; heads beyond the pass are zero.
   auto load_q = [&](int b, int hv) {
     const int h = hv / p.passes, pass = hv - h * p.passes;
     const int first = pass * p.per_pass;
     const int heads = min(p.per_pass, p.group - first);
-    const int my = kWide ? gid : gid & 3;
     const T* row = static_cast<const T*>(p.q) + static_cast<int64_t>(b) * p.q_stride +
-                   static_cast<int64_t>(h * p.group + first + my) * D + 4 * tig;
-    float x[C::kKK][8];
+                   static_cast<int64_t>(h * p.group + first + gid) * D + 4 * tig;
+    uint2 w[C::kKK];
     float amax = 0.f;
 #pragma unroll
     for (int kk = 0; kk < C::kKK; ++kk) {
+      w[kk] = make_uint2(0u, 0u);
+      if (gid < heads) w[kk] = __ldg(reinterpret_cast<const uint2*>(row + 16 * kk));
+      const T* e = reinterpret_cast<const T*>(&w[kk]);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint2 w = make_uint2(0u, 0u);
-        if (my < heads) w = __ldg(reinterpret_cast<const uint2*>(row + 32 * kk + 16 * half));
-        const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[kk][4 * half + i] = to_f32(e[i]);
-          amax = fmaxf(amax, fabsf(x[kk][4 * half + i]));
-        }
-      }
+      for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(to_f32(e[i])));
     }
     amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
@@ -381,56 +456,37 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     const float down = __uint_as_float(static_cast<uint32_t>(e - 7) << 23);
 #pragma unroll
     for (int kk = 0; kk < C::kKK; ++kk) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t part[kParts];
-        float r[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = x[kk][4 * half + i] * up;
-#pragma unroll
-        for (int j = 0; j < kParts; ++j) {
-          const uint32_t a = e4m3x2(r[0], r[1]), c = e4m3x2(r[2], r[3]);
-          part[j] = a | (c << 16);
-          const float2 fa = from_e4m3x2(a), fc = from_e4m3x2(c);
-          r[0] -= fa.x;
-          r[1] -= fa.y;
-          r[2] -= fc.x;
-          r[3] -= fc.y;
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if constexpr (kWide) qf[j][kk][half] = part[j];
-          else qf[j][kk][half] = gid < 4 ? part[2 * j] : (2 * j + 1 < kParts ? part[2 * j + 1 < kParts ? 2 * j + 1 : 0] : 0u);
-        }
-      }
+      const T* x = reinterpret_cast<const T*>(&w[kk]);
+      qf[kk][0] = MmaOp<__half>::pack(to_f32(x[0]) * up, to_f32(x[1]) * up);
+      qf[kk][1] = MmaOp<__half>::pack(to_f32(x[2]) * up, to_f32(x[3]) * up);
     }
-    f0 = __shfl_sync(kFull, down, 4 * head_a) * p.scale_log2;
-    f1 = __shfl_sync(kFull, down, 4 * (head_a + 1)) * p.scale_log2;
+    f0 = __shfl_sync(kFull, down, 8 * tig) * p.scale_log2;
+    f1 = __shfl_sync(kFull, down, 8 * tig + 4) * p.scale_log2;
   };
 
-  float o[C::kDT][4];
+  uint64_t o[C::kDT][2];  // (rows gid | gid + 8) x (columns 2 tig, 2 tig + 1)
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   int cb, chv, cu;
   locate(lo, cb, chv, cu);
   int cn = s_uoff[cb + 1] - s_uoff[cb];
-  int cctx = clamp_ctx(__ldg(p.ctx_lens + cb), max_tokens);
+  int cctx = s_ctx[cb];
   int64_t piece_start = lo;
   bool fresh = true, failed = false;
   int64_t pos = lo;
   int k = 0;
 
   auto finalize = [&](int64_t piece_end) {
+    float r[C::kDT][4];
+#pragma unroll
+    for (int dt = 0; dt < C::kDT; ++dt) {
+      unpack2(o[dt][0], r[dt][0], r[dt][1]);
+      unpack2(o[dt][1], r[dt][2], r[dt][3]);
+    }
     float t0 = l0, t1 = l1;
 #pragma unroll
     for (int x = 4; x < 32; x <<= 1) {
       t0 += __shfl_xor_sync(kFull, t0, x);
       t1 += __shfl_xor_sync(kFull, t1, x);
-    }
-    if constexpr (!kWide) {  // part 2's share of O sits in columns 4-7
-#pragma unroll
-      for (int dt = 0; dt < C::kDT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[dt][i] += __shfl_xor_sync(kFull, o[dt][i], 2);
     }
     const int h = chv / p.passes, pass = chv - h * p.passes;
     const int first = pass * p.per_pass;
@@ -439,20 +495,19 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     const int64_t seg_end = seg_start + cn;
     T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(cb) * p.out_stride +
              static_cast<int64_t>(h * p.group + first) * D;
-    const bool mine = kWide || first_part;
-    const int g0 = head_a, g1 = head_a + 1;
+    const int g0 = 2 * tig, g1 = 2 * tig + 1;
     if (piece_start == seg_start && piece_end == seg_end) {
       const float i0 = 1.f / t0, i1 = 1.f / t1;
 #pragma unroll
       for (int dt = 0; dt < C::kDT; ++dt) {
         const int d = 16 * dt + gid;
-        if (mine && g0 < heads) {
-          dst[g0 * D + d] = from_f32<T>(o[dt][0] * i0);
-          dst[g0 * D + d + 8] = from_f32<T>(o[dt][2] * i0);
+        if (g0 < heads) {
+          dst[g0 * D + d] = from_f32<T>(r[dt][0] * i0);
+          dst[g0 * D + d + 8] = from_f32<T>(r[dt][2] * i0);
         }
-        if (mine && g1 < heads) {
-          dst[g1 * D + d] = from_f32<T>(o[dt][1] * i1);
-          dst[g1 * D + d + 8] = from_f32<T>(o[dt][3] * i1);
+        if (g1 < heads) {
+          dst[g1 * D + d] = from_f32<T>(r[dt][1] * i1);
+          dst[g1 * D + d + 8] = from_f32<T>(r[dt][3] * i1);
         }
       }
       return;
@@ -463,16 +518,16 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
 #pragma unroll
     for (int dt = 0; dt < C::kDT; ++dt) {
       const int d = 16 * dt + gid;
-      if (mine && g0 < heads) {
-        wo[g0 * D + d] = o[dt][0];
-        wo[g0 * D + d + 8] = o[dt][2];
+      if (g0 < heads) {
+        wo[g0 * D + d] = r[dt][0];
+        wo[g0 * D + d + 8] = r[dt][2];
       }
-      if (mine && g1 < heads) {
-        wo[g1 * D + d] = o[dt][1];
-        wo[g1 * D + d + 8] = o[dt][3];
+      if (g1 < heads) {
+        wo[g1 * D + d] = r[dt][1];
+        wo[g1 * D + d + 8] = r[dt][3];
       }
     }
-    if (gid == 0 && mine) {
+    if (gid == 0) {
       float* wml = p.ws_ml + slot * kHeadsPad * 2;
       wml[g0 * 2] = m0;
       wml[g0 * 2 + 1] = t0;
@@ -499,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     if (fresh) {
       load_q(cb, chv);
 #pragma unroll
-      for (int dt = 0; dt < C::kDT; ++dt) o[dt][0] = o[dt][1] = o[dt][2] = o[dt][3] = 0.f;
+      for (int dt = 0; dt < C::kDT; ++dt) o[dt][0] = o[dt][1] = 0ull;
       m0 = m1 = -INFINITY;
       l0 = l1 = 0.f;
       piece_start = pos;
@@ -525,29 +580,53 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
       __syncwarp();
     }
 
-    // S^T in base-2 units, masked
-    float s[2][4];
+    // S^T in base-2 units. A warp has a scheduler to itself but for one other, so its own loads
+    // and MMAs have to overlap: all of K's fragments are fetched before the first is used, the
+    // MMAs run in four chains, and V's fragments are fetched under the softmax.
+    constexpr int kHalf = D == 256 ? 4 : C::kKK;  // k steps fetched at once
+    float s[2][4], c[2][2][4];
+    const uint32_t kbase = ktile + k_sw;
+#pragma unroll
+    for (int k0 = 0; k0 < C::kKK; k0 += kHalf) {
+      uint32_t x[2][kHalf / 2][4];
+#pragma unroll
+      for (int kk = 0; kk < kHalf; kk += 2)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+          ldmatrix_x4((kbase ^ sw(16 * (k0 + kk))) + 16 * mt * D, x[mt][kk / 2][0], x[mt][kk / 2][1],
+                      x[mt][kk / 2][2], x[mt][kk / 2][3]);
+#pragma unroll
+      for (int kk = 0; kk < kHalf; ++kk)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t a0, a1, a2, a3;
+          widen(x[mt][kk / 2][2 * (kk & 1)], a0, a2);
+          widen(x[mt][kk / 2][2 * (kk & 1) + 1], a1, a3);
+          if (k0 + kk < 2) mma_f16_zero(c[mt][kk & 1], a0, a1, a2, a3, qf[k0 + kk][0], qf[k0 + kk][1]);
+          else mma_f16(c[mt][kk & 1], a0, a1, a2, a3, qf[k0 + kk][0], qf[k0 + kk][1]);
+        }
+    }
+    constexpr int kAhead = D == 256 ? 4 : C::kDT;  // V tiles fetched at once
+    const uint32_t vbase = vtile + v_sw;
+    uint32_t y[kAhead][4];
+#pragma unroll
+    for (int dt = 0; dt < kAhead; ++dt)
+      ldmatrix_b8_trans_x2(vbase ^ sw(16 * dt), y[dt][0], y[dt][1], y[dt][2], y[dt][3]);
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kk = 0; kk < C::kKK; ++kk) {
-        uint32_t a0, a1, a2, a3;
-        ldmatrix_x4(ktile + sw(k_off + 16 * mt * D + 32 * kk), a0, a1, a2, a3);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) mma_e4m3(c, a0, a1, a2, a3, qf[j][kk][0], qf[j][kk][1]);
-      }
-      if constexpr (!kWide) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] += __shfl_xor_sync(kFull, c[i], 2);
-      }
       const float sk = (NP == 2 && mt == 1) ? scales.y : scales.x;
       const float a = f0 * sk, b = f1 * sk;
-      const bool v0 = 16 * mt + r0_tok < valid, v1 = 16 * mt + r1_tok < valid;
-      s[mt][0] = v0 ? c[0] * a : -INFINITY;
-      s[mt][1] = v0 ? c[1] * b : -INFINITY;
-      s[mt][2] = v1 ? c[2] * a : -INFINITY;
-      s[mt][3] = v1 ? c[3] * b : -INFINITY;
+      s[mt][0] = (c[mt][0][0] + c[mt][1][0]) * a;
+      s[mt][1] = (c[mt][0][1] + c[mt][1][1]) * b;
+      s[mt][2] = (c[mt][0][2] + c[mt][1][2]) * a;
+      s[mt][3] = (c[mt][0][3] + c[mt][1][3]) * b;
+    }
+    if (valid < kUnit) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        if (16 * mt + r0_tok >= valid) s[mt][0] = s[mt][1] = -INFINITY;
+        if (16 * mt + r1_tok >= valid) s[mt][2] = s[mt][3] = -INFINITY;
+      }
     }
     float u0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
     float u1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
@@ -565,60 +644,60 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     float sv = scales.z, w0 = 1.f, w1 = 1.f;
     if (NP == 2) {
       sv = fmaxf(scales.z, scales.w);
-      const float ratio = sv > 0.f ? fminf(scales.z, scales.w) / sv : 0.f;
+      const float ratio = sv > 0.f ? __fdividef(fminf(scales.z, scales.w), sv) : 0.f;
       w0 = scales.z == sv ? 1.f : ratio;
       w1 = scales.w == sv ? 1.f : ratio;
     }
-    uint32_t pb[NT][2];
+    uint32_t pb[2][2];
     float q0 = 0.f, q1 = 0.f;
+    const float s0 = u0 - 8.f, s1 = u1 - 8.f;
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      float e[4];
-      e[0] = fast_exp2(s[mt][0] - u0 + 8.f);
-      e[1] = fast_exp2(s[mt][1] - u1 + 8.f);
-      e[2] = fast_exp2(s[mt][2] - u0 + 8.f);
-      e[3] = fast_exp2(s[mt][3] - u1 + 8.f);
-      q0 += e[0] + e[2];
-      q1 += e[1] + e[3];
-      float part[kParts][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float r = NP == 2 ? e[i] * (mt ? w1 : w0) : e[i];
-#pragma unroll
-        for (int j = 0; j < kParts; ++j) {
-          part[j][i] = j + 1 < kParts ? round4(r) : r;
-          r -= part[j][i];
-        }
+      float e0 = fast_exp2(s[mt][0] - s0), e1 = fast_exp2(s[mt][1] - s1);
+      float e2 = fast_exp2(s[mt][2] - s0), e3 = fast_exp2(s[mt][3] - s1);
+      q0 += e0 + e2;
+      q1 += e1 + e3;
+      if (NP == 2) {
+        const float w = mt ? w1 : w0;
+        e0 *= w;
+        e1 *= w;
+        e2 *= w;
+        e3 *= w;
       }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (kWide) x[i] = part[j][i];
-          else x[i] = first_part ? part[2 * j][i] : (2 * j + 1 < kParts ? part[2 * j + 1 < kParts ? 2 * j + 1 : 0][i] : 0.f);
-        }
-        pb[j][mt] = movmatrix_trans(e4m3x2(x[0], x[2]) | (e4m3x2(x[1], x[3]) << 16));
-      }
+      pb[mt][0] = movmatrix_trans(MmaOp<__half>::pack(e0, e1));
+      pb[mt][1] = movmatrix_trans(MmaOp<__half>::pack(e2, e3));
     }
     l0 = l0 * al0 + be0 * q0;
     l1 = l1 * al1 + be1 * q1;
-    const float bs0 = be0 * sv, bs1 = be1 * sv;
+    const uint64_t al = pack2(al0, al1), bs = pack2(be0 * sv, be1 * sv);
 #pragma unroll
-    for (int dt = 0; dt < C::kDT; ++dt) {
-      uint32_t a0, a1, a2, a3;
-      ldmatrix_b8_trans_x2(vtile + sw(v_off + 16 * dt), a0, a1, a2, a3);
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int d0 = 0; d0 < C::kDT; d0 += kAhead) {
+      if (d0 > 0) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) mma_e4m3(c, a0, a1, a2, a3, pb[j][0], pb[j][1]);
-      o[dt][0] = o[dt][0] * al0 + c[0] * bs0;
-      o[dt][1] = o[dt][1] * al1 + c[1] * bs1;
-      o[dt][2] = o[dt][2] * al0 + c[2] * bs0;
-      o[dt][3] = o[dt][3] * al1 + c[3] * bs1;
+        for (int dt = 0; dt < kAhead; ++dt)
+          ldmatrix_b8_trans_x2(vbase ^ sw(16 * (d0 + dt)), y[dt][0], y[dt][1], y[dt][2], y[dt][3]);
+      }
+      float r[kAhead][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int dt = 0; dt < kAhead; ++dt) {
+          uint32_t a0, a1, a2, a3;
+          widen(y[dt][2 * mt], a0, a2);
+          widen(y[dt][2 * mt + 1], a1, a3);
+          if (mt == 0) mma_f16_zero(r[dt], a0, a1, a2, a3, pb[0][0], pb[0][1]);
+          else mma_f16(r[dt], a0, a1, a2, a3, pb[1][0], pb[1][1]);
+        }
+#pragma unroll
+      for (int dt = 0; dt < kAhead; ++dt) {
+        o[d0 + dt][0] = fma2(pack2(r[dt][0], r[dt][1]), bs, mul2(o[d0 + dt][0], al));
+        o[d0 + dt][1] = fma2(pack2(r[dt][2], r[dt][3]), bs, mul2(o[d0 + dt][1], al));
+      }
     }
     __syncwarp();
     if (issued < hi) {
       issue(issued, stage);
+      put_scales(issued, stage);
       ++issued;
     }
     ++k;
@@ -632,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
           do { ++cb; } while (cb < B && s_uoff[cb + 1] == s_uoff[cb]);
         }
         cn = s_uoff[cb + 1] - s_uoff[cb];
-        cctx = clamp_ctx(__ldg(p.ctx_lens + cb), max_tokens);
+        cctx = s_ctx[cb];
         fresh = true;
       }
     } else if (pos == hi) {
@@ -782,13 +861,14 @@ bool fast_shape(int dtype, int batch, int hkv, int group, int D, int S, int64_t 
          static_cast<int64_t>(batch) * hkv * ((group + 7) / 8) <= kMaxSegments &&
          pages * hkv * (S * D / 128) <= 0x7fffffff && pages * hkv <= 0x7fffffff && pages > 0 &&
          static_cast<int64_t>(max_pages) * S <= 0x7fffffff - kUnit &&
-         // positions of the unit stream times warps stay far inside 64 bits, counts inside 32
-         static_cast<int64_t>(batch) * ((static_cast<int64_t>(max_pages) * S + kUnit - 1) / kUnit) <= 0x7fffffff;
+         // units are counted in 32 bits
+         static_cast<int64_t>(batch) * ((static_cast<int64_t>(max_pages) * S + kUnit - 1) / kUnit) * hkv *
+                 ((group + 7) / 8) < 0x70000000;
 }
 
-template <typename T, int D, int S, bool kWide>
+template <typename T, int D, int S>
 int launch(const Params& p, const void* k_pool, const void* v_pool, cudaStream_t stream) {
-  auto kern = decode_q8_kernel<T, D, S, kWide>;
+  auto kern = decode_q8_kernel<T, D, S>;
   static std::atomic<int> configured[64];  // CTAs per SM + 1, per device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return PI_ERR_CUDA;
@@ -801,6 +881,7 @@ int launch(const Params& p, const void* k_pool, const void* v_pool, cudaStream_t
     configured[dev].store(1, std::memory_order_release);
   }
   // two CTAs share an SM while the prefix table leaves room for both
+  // two CTAs share an SM while the tables leave room for both
   const int per_sm = D <= 128 && 2 * (smem + 1024) <= 228 * 1024 ? 2 : 1;
   const uint64_t rows = static_cast<uint64_t>(p.num_pages) * p.hkv * (S * D / 128);
   CUtensorMap tk, tv;
@@ -879,10 +960,8 @@ extern "C" int pi_paged_decode_attn_q8(void* out, const void* q, const void* k_p
     p.ws_cnt = reinterpret_cast<int*>(ws);
     p.ws_ml = reinterpret_cast<float*>(ws + L.ml_off);
     p.ws_o = reinterpret_cast<float*>(ws + L.o_off);
-#define PI_Q8(T, D, S)                                                                         \
-  if (head_dim == D && page_size == S)                                                         \
-    return p.per_pass > 4 ? q8::launch<T, D, S, true>(p, k_pool, v_pool, stream)               \
-                          : q8::launch<T, D, S, false>(p, k_pool, v_pool, stream);
+#define PI_Q8(T, D, S) \
+  if (head_dim == D && page_size == S) return q8::launch<T, D, S>(p, k_pool, v_pool, stream);
 #define PI_Q8_ALL(T) PI_Q8(T, 64, 16) PI_Q8(T, 64, 32) PI_Q8(T, 128, 16) PI_Q8(T, 128, 32) \
                      PI_Q8(T, 256, 16) PI_Q8(T, 256, 32)
     if (dtype == PI_DTYPE_BF16) { PI_Q8_ALL(__nv_bfloat16) } else { PI_Q8_ALL(__half) }
@@ -901,3 +980,4 @@ extern "C" int pi_paged_decode_attn_q8(void* out, const void* q, const void* k_p
       return cuda_status(launch_kernel(q8::decode_q8_generic_kernel<__half>, grid, dim3(128), 0, stream, p, kp, vp, head_dim, page_size));
   }
 }
+

@@ -36,7 +36,6 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kMinExp = -118;  // smallest scale exponent: 2^e and 2^-e are normal floats
-constexpr float kE4m3Max = 448.f;
 
 struct AppendParams {
   void* q_out;

@@ -72,6 +72,28 @@ def test_decode_many_requests_and_one_long(dtype):
         check(attend(q, c), ref, tol)
 
 
+@pytest.mark.parametrize("dtype,G,D,S", [("bf16", 4, 64, 16), ("f16", 8, 128, 32), ("bf16", 2, 256, 16)])
+def test_decode_long_streams(dtype, G, D, S):
+    # enough units that a part of the stream is handed out in chunks, and every stage of the rings
+    # goes round many times; lengths from nothing to many times a CTA's share
+    lens = [9000, 1, 0, 4500, 12001, 33, 7000, 5000, 3000, 640]
+    c = on_gpu(cache(lens, 8, D, S, seed=14))
+    q = queries(len(lens), 8 * G, D, dtype, 14)
+    ref, tol = reference(q, c, lens)
+    first = attend(q, c)
+    check(first, ref, tol)
+    for _ in range(5):  # whoever computes which chunk, the result is the same
+        assert torch.equal(attend(q, c), first)
+
+
+def test_decode_more_requests_than_one_launch():
+    lens = [int(x) for x in np.random.default_rng(1).integers(0, 60, 2100)]
+    c = on_gpu(cache(lens, 1, 64, 16, seed=15))
+    q = queries(len(lens), 2, 64, "bf16", 15)
+    ref, tol = reference(q, c, lens)
+    check(attend(q, c), ref, tol)
+
+
 @pytest.mark.parametrize("plain_scales", [False, True])
 def test_decode_scales(plain_scales):
     # neighbouring pages whose scales differ by many powers of two; scales that are no powers
