@@ -507,6 +507,37 @@ int pi_paged_decode_attn_q8(void* out, const void* q, const void* k_pool, const 
                             cudaStream_t stream);
 
 /*
+ * pi_paged_prefill_attn over an 8-bit cache (arguments and mask as there, pools and scales as
+ * in pi_paged_decode_attn_q8): several query tokens of one request, causal with an offset or
+ * not. Any head ratio; q and out of f32, bf16 or f16; head_dim <= 256. Rows that see no key are
+ * zero. Many query rows: the pages are widened into `workspace` in q's type (exact in bf16 for
+ * power-of-two scales; an f16 value past 65504 becomes 65504) and pi_paged_prefill_attn_tc runs
+ * on them; few, or shapes that it does not take: the kernels of pi_paged_decode_attn_q8.
+ *   workspace   pi_paged_prefill_attn_q8_workspace_bytes(...) bytes; it begins with the
+ *               scratch of pi_paged_decode_attn_q8, whose zeroed part is as there
+ */
+size_t pi_paged_prefill_attn_q8_workspace_bytes(int q_len, int kv_len, int num_q_heads,
+                                                int num_kv_heads, int head_dim, int page_size,
+                                                int dtype);
+int pi_paged_prefill_attn_q8(void* out, const void* q, const void* k_pool, const void* v_pool,
+                             const float* k_scale, const float* v_scale,
+                             const int32_t* block_table, int64_t table_len, int q_len, int kv_len,
+                             int q_start, int causal, int num_q_heads, int num_kv_heads,
+                             int head_dim, int page_size, int64_t num_pages, float scale, int dtype,
+                             int64_t q_tok_stride, int64_t out_tok_stride, void* workspace,
+                             size_t workspace_bytes, int* err, cudaStream_t stream);
+
+/*
+ * Pages of an 8-bit pool widened to `dtype` (f32, bf16 or f16):
+ *   out[i, h, s, :] = pool[page_ids[i], h, s, :] * scale[page_ids[i], h]   out [n, kv_heads, S, D]
+ * one rounding (none in bf16 for power-of-two scales); an f16 value past 65504 becomes 65504.
+ * A page id outside the pool gives zeros and is reported through `err`.
+ */
+int pi_page_dequant(void* out, const void* pool, const float* scale, const int32_t* page_ids,
+                    int64_t n_pages, int kv_heads, int head_dim, int page_size, int64_t num_pages,
+                    int dtype, int* err, cudaStream_t stream);
+
+/*
  * Contiguous gather of a request's pages in the reference's gather layout:
  *   out[t, h, :] = pool[block_table[t / page_size], h, t % page_size, :]
  * for t in [0, num_tokens). out is [num_tokens, kv_heads, head_dim].

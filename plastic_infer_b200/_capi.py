@@ -126,6 +126,19 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i64,
          _f32, _i32, _i64, _i64, _vp, _sz, _vp, _vp],
     ),
+    # q_len, kv_len, hq, hkv, head_dim, page_size, dtype
+    "pi_paged_prefill_attn_q8_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    # out, q, k_pool, v_pool, k_scale, v_scale, block_table, table_len, q_len, kv_len, q_start,
+    # causal, hq, hkv, head_dim, page_size, num_pages, scale, dtype, q_tok_stride,
+    # out_tok_stride, workspace, workspace_bytes, err, stream
+    "pi_paged_prefill_attn_q8": (
+        _i32,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+         _i64, _f32, _i32, _i64, _i64, _vp, _sz, _vp, _vp],
+    ),
+    # out, pool, scale, page_ids, n_pages, kv_heads, head_dim, page_size, num_pages, dtype, err,
+    # stream
+    "pi_page_dequant": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _i32, _vp, _vp]),
     # q_len, num_q_heads, num_kv_heads, head_dim, kv_len
     "pi_host_stream_attn_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i64]),
     # out, q, q_tok_stride, out_tok_stride, spans (host array), num_spans, q_len, q_start,

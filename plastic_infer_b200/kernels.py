@@ -22,6 +22,9 @@ These are the batched additions behind the reference's single-request API:
   rope_frequencies       rotary frequencies for rope_append: plain, or scaled for long contexts
   paged_decode_attention_q8
                          decode attention over e4m3 pools with a scale per (page, KV head)
+  paged_prefill_attention_q8
+                         several query tokens of one request over such pools
+  page_dequant           pages of such a pool widened to f32, bf16 or f16
   paged_prefill_attention
                          one request's prefill straight from the pool
                          (reference: _attn_paged, src/plastic_infer/exec/runner_paged.py:36-95)
@@ -640,7 +643,7 @@ def paged_decode_attention(
 # ---------------------------------------------------------------------------
 
 _q8_ws: dict[tuple[int, int], Workspace] = {}
-_q8_ws_bytes: dict[tuple[int, int], int] = {}
+_q8_decode_bytes: dict[tuple[int, int], int] = {}
 
 
 def _check_q8_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
@@ -654,16 +657,10 @@ def _check_q8_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.T
     return P, Hkv, S, D
 
 
-def _q8_workspace(device: torch.device, head_dim: int, workspace: Workspace | None) -> torch.Tensor:
+def _q8_workspace(device: torch.device, nbytes: int, workspace: Workspace | None) -> torch.Tensor:
     """Scratch for one q8 attention call on the device's current stream: the caller's, or one
     of the stream's own, so that calls on two streams never share it. Under graph capture it
     comes out of the graph's memory, zeroed by the graph: no two graphs share it either."""
-    key = (device.index, head_dim)
-    nbytes = _q8_ws_bytes.get(key)
-    if nbytes is None:
-        with torch.cuda.device(device):
-            nbytes = int(_capi.load().pi_paged_decode_attn_q8_workspace_bytes(head_dim))
-        _q8_ws_bytes[key] = nbytes
     if workspace is not None:
         if torch.device(workspace.device).index not in (None, device.index):
             raise ValueError(f"the workspace is on {workspace.device}, q on {device}")
@@ -678,6 +675,16 @@ def _q8_workspace(device: torch.device, head_dim: int, workspace: Workspace | No
         with _ws_lock:
             ws = _q8_ws.setdefault(stream, Workspace(device))
     return ws.get(nbytes)
+
+
+def _q8_decode_workspace_bytes(device: torch.device, head_dim: int) -> int:
+    key = (device.index, head_dim)
+    nbytes = _q8_decode_bytes.get(key)
+    if nbytes is None:
+        with torch.cuda.device(device):
+            nbytes = int(_capi.load().pi_paged_decode_attn_q8_workspace_bytes(head_dim))
+        _q8_decode_bytes[key] = nbytes
+    return nbytes
 
 
 def paged_decode_attention_q8(
@@ -728,7 +735,7 @@ def paged_decode_attention_q8(
         return out
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    ws = _q8_workspace(device, D, workspace)
+    ws = _q8_workspace(device, _q8_decode_workspace_bytes(device, D), workspace)
     row = Hq * D
     _call_on(
         device, "pi_paged_decode_attn_q8",
@@ -738,6 +745,102 @@ def paged_decode_attention_q8(
         q.stride(0) if B > 1 else row, out.stride(0) if B > 1 else row, ws.data_ptr(), ws.numel(),
         _err_ptr(err),
     )
+    return out
+
+
+def paged_prefill_attention_q8(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    kv_len: int,
+    q_start: int = 0,
+    causal: bool = True,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+    workspace: Workspace | None = None,
+    err: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of one request's q [q_len, Hq, D] (or [1, q_len, Hq, D]) over the first kv_len
+    tokens of its pages in an 8-bit cache (pools and scales as in paged_decode_attention_q8).
+
+    Query i sits at position q_start + i; with `causal` it sees keys j <= q_start + i. Returns
+    [q_len, Hq, D] in q's dtype (the input's leading batch axis is kept when given). Long chunks
+    widen the request's pages once into the workspace and run the tcgen05 prefill on them; short
+    ones, and shapes that it does not take, run the 8-bit decode kernels over several rows.
+    """
+    P, Hkv, S, D = _check_q8_pools(k_pool, v_pool, k_scale, v_scale)
+    batched = q.dim() == 4
+    if batched and q.shape[0] != 1:
+        raise ValueError("prefill attends one request: q must be [1, q_len, Hq, D]")
+    q3 = q[0] if batched else q
+    if q3.dim() != 3 or q3.shape[2] != D:
+        raise ValueError(f"q must be [q_len, Hq, {D}]")
+    n, Hq = q3.shape[0], q3.shape[1]
+    if Hq == 0 or Hq % Hkv != 0:
+        raise ValueError(f"num_q_heads {Hq} not a multiple of num_kv_heads {Hkv}")
+    code = dtype_code(q3.dtype)
+    if block_table.dtype != torch.int32 or block_table.dim() != 1:
+        raise ValueError("block_table must be int32 [n]")
+    kv_len, q_start = int(kv_len), int(q_start)
+    if kv_len > block_table.numel() * S or kv_len < 0 or q_start < 0 or q_start + n > 2 ** 31 - 1:
+        raise ValueError("kv_len must be within the block table's pages, q_start not negative")
+    device = _check_one_device(q3, k_pool, v_pool, k_scale, v_scale, block_table, out, err)
+    if q3.stride(2) != 1 or q3.stride(1) != D or (n > 1 and q3.stride(0) < Hq * D):
+        q3 = q3.contiguous()
+    block_table = block_table.contiguous()
+    if out is None:
+        out3 = torch.empty((n, Hq, D), dtype=q3.dtype, device=device)
+    else:
+        out3 = out[0] if out.dim() == 4 else out
+        if out3.shape != (n, Hq, D) or out3.dtype != q3.dtype or out3.stride(2) != 1 \
+                or out3.stride(1) != D:
+            raise ValueError("out must be [q_len, Hq, D] in q's dtype with contiguous heads")
+    if n > 0:
+        if scale is None:
+            scale = 1.0 / math.sqrt(D)
+        with torch.cuda.device(device):
+            nbytes = int(_capi.load().pi_paged_prefill_attn_q8_workspace_bytes(
+                n, kv_len, Hq, Hkv, D, S, code))
+        ws = _q8_workspace(device, nbytes, workspace)
+        row = Hq * D
+        _call_on(
+            device, "pi_paged_prefill_attn_q8",
+            out3.data_ptr(), q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), block_table.numel(), n,
+            kv_len, q_start, 1 if causal else 0, Hq, Hkv, D, S, P, float(scale), code,
+            q3.stride(0) if n > 1 else row, out3.stride(0) if n > 1 else row, ws.data_ptr(),
+            ws.numel(), _err_ptr(err),
+        )
+    if out is not None:
+        return out
+    return out3.unsqueeze(0) if batched else out3
+
+
+def page_dequant(pool: torch.Tensor, scale: torch.Tensor, page_ids: torch.Tensor,
+                 dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+                 err: torch.Tensor | None = None) -> torch.Tensor:
+    """out[i, h] = pool[page_ids[i], h] * scale[page_ids[i], h]: pages of an 8-bit pool widened to
+    `dtype` (f32, bf16 or f16), [n, Hkv, page_size, D]. Exact in bf16 and f32 for power-of-two
+    scales; an f16 value past 65504 becomes 65504."""
+    P, Hkv, S, D = _check_pool(pool, "pool")
+    if pool.dtype != torch.float8_e4m3fn:
+        raise TypeError("the pool must be torch.float8_e4m3fn")
+    _check_scales(scale, scale, P, Hkv)
+    if page_ids.dtype != torch.int32 or page_ids.dim() != 1:
+        raise ValueError("page_ids must be int32 [n]")
+    code = dtype_code(dtype)
+    n = page_ids.numel()
+    device = _check_one_device(pool, scale, page_ids, out, err)
+    if out is None:
+        out = torch.empty((n, Hkv, S, D), dtype=dtype, device=device)
+    elif out.dtype != dtype or tuple(out.shape) != (n, Hkv, S, D) or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous [{n}, {Hkv}, {S}, {D}] {dtype}")
+    if n:
+        _call_on(device, "pi_page_dequant", out.data_ptr(), pool.data_ptr(), scale.data_ptr(),
+                 page_ids.contiguous().data_ptr(), n, Hkv, D, S, P, code, _err_ptr(err))
     return out
 
 

@@ -74,3 +74,82 @@ def test_decode_c_entry_validates_before_launch():
     need = lib.pi_paged_decode_attn_q8_workspace_bytes(128)
     assert rc(_20=ctypes.c_void_p(128), _21=need) == _capi.PI_ERR_MISALIGNED
     assert lib.pi_paged_decode_attn_q8_ws_zero_bytes() < need
+
+
+def _chunk(n=2, **kw):
+    a = _args(B=n)
+    a.pop("ctx_lens")
+    a["block_table"] = a.pop("block_tables")[0]
+    return {**a, "kv_len": 20, **kw}
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(q=torch.zeros(2, 2, 4, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(q=torch.zeros(2, 4, 32, dtype=torch.bfloat16)), ValueError),
+    (dict(q=torch.zeros(2, 3, 64, dtype=torch.bfloat16)), ValueError),
+    (dict(k_pool=torch.zeros(4, 2, 16, 64)), TypeError),
+    (dict(k_scale=torch.zeros(2, 4)), ValueError),
+    (dict(block_table=torch.zeros(3, dtype=torch.int64)), ValueError),
+    (dict(block_table=torch.zeros(1, 3, dtype=torch.int32)), ValueError),
+    (dict(kv_len=49), ValueError),
+    (dict(kv_len=-1), ValueError),
+    (dict(q_start=-1), ValueError),
+    (dict(q_start=2 ** 31), ValueError),
+    (dict(), ValueError),
+])
+def test_prefill_refuses(change, error):
+    with pytest.raises(error):
+        kernels.paged_prefill_attention_q8(**{**_chunk(), **change})
+
+
+@pytest.mark.parametrize("args,error", [
+    ((torch.zeros(4, 2, 16, 64), torch.zeros(4, 2), torch.zeros(1, dtype=torch.int32)), TypeError),
+    ((torch.zeros(4, 2, 16, 64).to(E4M3), torch.zeros(4, 3), torch.zeros(1, dtype=torch.int32)), ValueError),
+    ((torch.zeros(4, 2, 16, 64).to(E4M3), torch.zeros(4, 2), torch.zeros(1, dtype=torch.int64)), ValueError),
+    ((torch.zeros(4, 2, 16, 64).to(E4M3), torch.zeros(4, 2), torch.zeros(1, dtype=torch.int32),
+      torch.float64), TypeError),
+    ((torch.zeros(4, 2, 16, 64).to(E4M3), torch.zeros(4, 2), torch.zeros(1, dtype=torch.int32)), ValueError),
+])
+def test_page_dequant_refuses(args, error):
+    with pytest.raises(error):
+        kernels.page_dequant(*args)
+
+
+def test_prefill_c_entries_validate_before_launch():
+    _build.build()
+    lib = _capi.load()
+    a = ctypes.c_void_p(256)
+    # out, q, k_pool, v_pool, k_scale, v_scale, table, table_len, q_len, kv_len, q_start, causal, hq,
+    # hkv, d, s, pages, scale, dtype, q_stride, out_stride, workspace, bytes, err, stream
+    base = [a, a, a, a, a, a, a, 4, 3, 40, 0, 1, 4, 2, 128, 16, 8, 1.0, _capi.PI_DTYPE_BF16, 512, 512, None, 0,
+            None, None]
+
+    def rc(**change):
+        x = list(base)
+        for i, v in change.items():
+            x[int(i[1:])] = v
+        return lib.pi_paged_prefill_attn_q8(*x)
+
+    assert rc(_8=0) == _capi.PI_OK
+    assert rc(_18=_capi.PI_DTYPE_E4M3) == _capi.PI_ERR_UNSUPPORTED
+    assert rc(_14=264, _19=4096, _20=4096) == _capi.PI_ERR_UNSUPPORTED
+    for change in (dict(_8=-1), dict(_9=65), dict(_9=-1), dict(_10=-1), dict(_12=5), dict(_19=511), dict(_20=511),
+                   dict(_10=2 ** 31 - 2)):
+        assert rc(**change) == _capi.PI_ERR_BAD_SHAPE, change
+    for i in range(7):
+        assert rc(**{f"_{i}": None}) == _capi.PI_ERR_NULL_POINTER, i
+    for i in (0, 1, 4, 5, 6):
+        assert rc(**{f"_{i}": ctypes.c_void_p(257)}) == _capi.PI_ERR_MISALIGNED, i
+    assert rc() == _capi.PI_ERR_WORKSPACE
+    assert rc(_8=4000) == _capi.PI_ERR_WORKSPACE
+    need = lib.pi_paged_prefill_attn_q8_workspace_bytes
+    few = need(3, 40, 4, 2, 128, 16, _capi.PI_DTYPE_BF16)
+    assert few == lib.pi_paged_decode_attn_q8_workspace_bytes(128)
+    assert need(4000, 40, 4, 2, 128, 16, _capi.PI_DTYPE_BF16) >= few + 2 * 3 * 2 * 16 * 128 * 2
+    assert need(4000, 40, 4, 2, 128, 16, _capi.PI_DTYPE_F32) == few
+    d = lib.pi_page_dequant
+    assert d(a, a, a, a, 0, 2, 128, 16, 8, 1, None, None) == _capi.PI_OK
+    assert d(a, a, a, a, 1, 2, 128, 16, 8, 7, None, None) == _capi.PI_ERR_UNSUPPORTED
+    assert d(a, a, a, a, -1, 2, 128, 16, 8, 1, None, None) == _capi.PI_ERR_BAD_SHAPE
+    assert d(a, None, a, a, 1, 2, 128, 16, 8, 1, None, None) == _capi.PI_ERR_NULL_POINTER
+    assert d(a, a, ctypes.c_void_p(257), a, 1, 2, 128, 16, 8, 1, None, None) == _capi.PI_ERR_MISALIGNED
