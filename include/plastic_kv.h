@@ -507,6 +507,12 @@ int pi_paged_decode_attn_q8(void* out, const void* q, const void* k_pool, const 
                             cudaStream_t stream);
 
 /*
+ * Query rows (q_len x num_q_heads) up to which pi_paged_prefill_attn_q8 keeps to the decode
+ * kernels; the workspace is then pi_paged_decode_attn_q8_workspace_bytes(head_dim).
+ */
+#define PI_Q8_FEW_ROWS 5120
+
+/*
  * pi_paged_prefill_attn over an 8-bit cache (arguments and mask as there, pools and scales as
  * in pi_paged_decode_attn_q8): several query tokens of one request, causal with an offset or
  * not. Any head ratio; q and out of f32, bf16 or f16; head_dim <= 256. Rows that see no key are

@@ -153,6 +153,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pi_page_scatter": (_i32, [_vp, _vp, _vp, _i64, _i32, _i64, _i32, _i64, _vp, _vp]),
 }
 
+Q8_FEW_ROWS = 5120  # PI_Q8_FEW_ROWS
+
 MAX_PEERS = 8  # PI_MAX_PEERS
 
 

@@ -1242,12 +1242,11 @@ WideLayout wide_layout(int64_t pages, int hkv, int D, int S) {
   return w;
 }
 
-// Many query rows: the pages are widened once into scratch and the tcgen05 prefill runs on them. Few:
-// the rows ride in the decode kernel, 16 to a pass over the cache (from L2 after the first).
-// PI_Q8_FEW_ROWS: query rows times KV heads up to which the second was faster.
-#ifndef PI_Q8_FEW_ROWS
-#define PI_Q8_FEW_ROWS 5120
-#endif
+// Many query rows (above PI_Q8_FEW_ROWS): the pages are widened once into scratch and the tcgen05 prefill
+// runs on them. Few: the rows ride in the decode kernel, 16 to a pass over the cache (from L2 after
+// the first). Measured after 8000 tokens, 32/8 heads of 128: 64 / 128 / 160 / 256 queries take 66 /
+// 123 / 144 / 207 us in passes and 154 / 156 / 154 / 153 us widened; with 4 query heads on one KV
+// head 128 / 512 queries after 16000 take 41 / 111 us against 270 / 275.
 bool widens(int q_len, int kv_len, int hq, int hkv, int D, int S, int dtype) {
   const int G = hq / hkv;
   return (dtype == PI_DTYPE_BF16 || dtype == PI_DTYPE_F16) && (D == 64 || D == 128) && (S == 16 || S == 32) &&

@@ -301,22 +301,24 @@ def _check_one_device(*tensors: torch.Tensor | None) -> torch.device:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            _require_cuda(t)
         if device is None:
             device = t.device
+            if device.type != "cuda":
+                _require_cuda(t)
         elif t.device != device:
+            _require_cuda(t)
             raise ValueError(f"all tensors must be on one device, got {device} and {t.device}")
     return device  # type: ignore[return-value]
 
 
 def _call_on(device: torch.device, func: str, *args) -> None:
     """_capi.call on the current stream of `device`, with that device current."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if device.index == torch.cuda.current_device():
-        _capi.call(func, *args, torch.cuda.current_stream(device).cuda_stream)
+        _capi.call(func, *args, stream)
         return
     with torch.cuda.device(device):
-        _capi.call(func, *args, torch.cuda.current_stream(device).cuda_stream)
+        _capi.call(func, *args, stream)
 
 
 def rope_append(
@@ -669,7 +671,7 @@ def _q8_workspace(device: torch.device, nbytes: int, workspace: Workspace | None
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         buf[:int(_capi.load().pi_paged_decode_attn_q8_ws_zero_bytes())].zero_()
         return buf
-    stream = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    stream = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
     ws = _q8_ws.get(stream)
     if ws is None:
         with _ws_lock:
@@ -801,9 +803,11 @@ def paged_prefill_attention_q8(
     if n > 0:
         if scale is None:
             scale = 1.0 / math.sqrt(D)
-        with torch.cuda.device(device):
-            nbytes = int(_capi.load().pi_paged_prefill_attn_q8_workspace_bytes(
-                n, kv_len, Hq, Hkv, D, S, code))
+        nbytes = _q8_decode_workspace_bytes(device, D)
+        if n * Hq > _capi.Q8_FEW_ROWS:  # (fewer rows need the decode scratch only)
+            with torch.cuda.device(device):
+                nbytes = int(_capi.load().pi_paged_prefill_attn_q8_workspace_bytes(
+                    n, kv_len, Hq, Hkv, D, S, code))
         ws = _q8_workspace(device, nbytes, workspace)
         row = Hq * D
         _call_on(

@@ -147,6 +147,8 @@ def test_prefill_c_entries_validate_before_launch():
     assert few == lib.pi_paged_decode_attn_q8_workspace_bytes(128)
     assert need(4000, 40, 4, 2, 128, 16, _capi.PI_DTYPE_BF16) >= few + 2 * 3 * 2 * 16 * 128 * 2
     assert need(4000, 40, 4, 2, 128, 16, _capi.PI_DTYPE_F32) == few
+    edge = _capi.Q8_FEW_ROWS // 4  # the wrapper asks for more from here on
+    assert need(edge, 40, 4, 2, 128, 16, _capi.PI_DTYPE_BF16) == few < need(edge + 1, 40, 4, 2, 128, 16, _capi.PI_DTYPE_BF16)
     d = lib.pi_page_dequant
     assert d(a, a, a, a, 0, 2, 128, 16, 8, 1, None, None) == _capi.PI_OK
     assert d(a, a, a, a, 1, 2, 128, 16, 8, 7, None, None) == _capi.PI_ERR_UNSUPPORTED
