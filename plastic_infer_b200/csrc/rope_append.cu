@@ -27,7 +27,7 @@
 // apart in the half layout, adjacent in the interleaved one.
 //
 // Measured on B200 (32 query and 8 KV heads of 128, bf16, QK-norm): 8192 tokens in 54 us, 3.8 TB/s,
-// 0.57 of the measured copy rate; into e4m3 pools 78 us, 0.36 (a block's two barriers and its
+// 0.57 of the measured copy rate; into e4m3 pools 76 us, 0.37 (a block's two barriers and its
 // maximum before anything is written). Two rows' loads in flight per lane were slower (72 us: 80
 // registers instead of 56 leave fewer warps). 64 tokens take 6.4 and 8.4 us in a graph.
 #include <type_traits>
@@ -145,12 +145,18 @@ __device__ __forceinline__ void norm_rotate(float (&x)[16], const LaneCols& c, c
     for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
 #pragma unroll
     for (int o = L / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float rinv = 1.f / sqrtf(ss / static_cast<float>(16 * L) + eps);
+    // x / rms with the quotient's residual put back: a value next to an e4m3 border should not cross
+    // it for two roundings more
+    const float rms = sqrtf(ss / static_cast<float>(16 * L) + eps);
+    const float rinv = 1.f / rms;
     float wv[16];
     load8(w + c.a, wv);
     load8(w + c.b, wv + 8);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = x[i] * rinv * wv[i];
+    for (int i = 0; i < 16; ++i) {
+      const float y = x[i] * rinv;
+      x[i] = fmaf(fmaf(-y, rms, x[i]), rinv, y) * wv[i];
+    }
   }
   if (c.pair < 0) return;
   const float4* t = reinterpret_cast<const float4*>(table + c.pair);  // two (cos, sin) pairs each

@@ -348,7 +348,7 @@ def rope_append(
     < 0: no K/V row). inv_freq fp32 [R / 2] turns the first R elements of a head
     (rope_frequencies): pairs (j, j + R/2), or (2j, 2j + 1) with `interleaved`; rope_scale
     multiplies cosine and sine. Angles are formed in 64 bits, so far positions keep their
-    precision. Returns q_out [T, Hq, D].
+    precision. Returns q_out [T, Hq, D], which must not overlap the inputs.
 
     16/32-bit pools take the rows in the pool dtype, which is q_out's too. Pools of
     torch.float8_e4m3fn need k_scale and v_scale, fp32 [num_pages, Hkv] (q_out then has q's
