@@ -251,9 +251,11 @@ def rope_frequencies(rotary_dim: int, base: float, scaling: str = "none", factor
     "linear"  every frequency divided by `factor` (positions interpolated)
     "ntk"     base raised to base * factor^(R / (R - 2)): the slowest pair is stretched by
               `factor`, the fastest not at all
-    "yarn"    pairs that turn fewer than beta_slow times in the trained length are divided by
-              `factor`, those that turn more than beta_fast times are kept, a linear ramp over
-              the pair index in between; rope_scale = 0.1 ln(factor) + 1
+    "yarn"    (Peng et al., "YaRN: Efficient Context Window Extension of Large Language Models",
+              2023) pairs that turn fewer than beta_slow times in the trained length are divided
+              by `factor`, those that turn more than beta_fast times are kept, a linear ramp over
+              the pair index in between, which may end past the last pair;
+              rope_scale = 0.1 ln(factor) + 1
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be positive and even, got {rotary_dim}")
@@ -278,7 +280,7 @@ def rope_frequencies(rotary_dim: int, base: float, scaling: str = "none", factor
                     / (2 * math.log(base)))
 
         low = max(math.floor(pair_turning(beta_fast)), 0)
-        high = min(math.ceil(pair_turning(beta_slow)), rotary_dim // 2 - 1)
+        high = min(math.ceil(pair_turning(beta_slow)), rotary_dim - 1)
         ramp = (torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)
         keep = 1.0 - ramp.clamp(0, 1)
         inv = inv / factor * (1 - keep) + inv * keep
