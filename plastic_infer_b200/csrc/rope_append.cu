@@ -135,6 +135,25 @@ __device__ __forceinline__ void store8_e4m3(uint8_t* p, const float* x, float in
                  e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv));
 }
 
+// Division by the root mean square of a row. x * rinv is a rounding off the quotient twice over; with
+// its residual x - y rms put back (one Newton step on the quotient) it is the quotient rounded once in
+// all but rare cases, which keeps a value next to an e4m3 border on its side. A root that overflowed
+// (an infinity in the row, or a sum of squares past fp32) or is 0 has no residual: x / inf = 0 for
+// every finite x, inf / inf = NaN, as the division itself gives.
+struct RowNorm {
+  float rms, rinv;
+  bool exact;
+};
+
+__device__ __forceinline__ RowNorm row_norm(float mean_square, float eps) {
+  const float rms = sqrtf(mean_square + eps);
+  return {rms, 1.f / rms, rms > 0.f && rms < INFINITY};
+}
+
+__device__ __forceinline__ float put_back(float x, float y, const RowNorm& n) {
+  return fmaf(fmaf(-y, n.rms, x), n.rinv, y);
+}
+
 // Norm (over the row's L lanes; every lane of the warp calls) and rotation in place.
 template <typename Ti, int L>
 __device__ __forceinline__ void norm_rotate(float (&x)[16], const LaneCols& c, const Ti* w,
@@ -145,17 +164,14 @@ __device__ __forceinline__ void norm_rotate(float (&x)[16], const LaneCols& c, c
     for (int i = 0; i < 16; ++i) ss += x[i] * x[i];
 #pragma unroll
     for (int o = L / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    // x / rms with the quotient's residual put back: a value next to an e4m3 border should not cross
-    // it for two roundings more
-    const float rms = sqrtf(ss / static_cast<float>(16 * L) + eps);
-    const float rinv = 1.f / rms;
+    const RowNorm n = row_norm(ss / static_cast<float>(16 * L), eps);
     float wv[16];
     load8(w + c.a, wv);
     load8(w + c.b, wv + 8);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float y = x[i] * rinv;
-      x[i] = fmaf(fmaf(-y, rms, x[i]), rinv, y) * wv[i];
+      const float y = x[i] * n.rinv;
+      x[i] = (n.exact ? put_back(x[i], y, n) : y) * wv[i];
     }
   }
   if (c.pair < 0) return;
@@ -421,11 +437,16 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const AppendParam
 // Any other shape, alignment or page size: one element at a time, one warp per row.
 // ---------------------------------------------------------------------------------------
 
-// Element d of the (normed, rotated) row; rinv is 1 / rms, or 1 without a norm.
+// Element d of the (normed, rotated) row; `norm` is not looked at without weights.
 template <typename Ti>
-__device__ float rotated_element(const AppendParams& p, const Ti* src, const Ti* w, float rinv,
+__device__ float rotated_element(const AppendParams& p, const Ti* src, const Ti* w, const RowNorm& norm,
                                  int64_t pos, int d) {
-  auto at = [&](int i) { return to_f32(src[i]) * (w ? rinv * to_f32(w[i]) : 1.f); };
+  auto at = [&](int i) {
+    const float x = to_f32(src[i]);
+    if (w == nullptr) return x;
+    const float y = x * norm.rinv;
+    return (norm.exact ? put_back(x, y, norm) : y) * to_f32(w[i]);
+  };
   const int n = p.pairs;
   if (d >= 2 * n) return at(d);
   const int j = p.interleaved ? d / 2 : (d < n ? d : d - n);
@@ -436,8 +457,8 @@ __device__ float rotated_element(const AppendParams& p, const Ti* src, const Ti*
 }
 
 template <typename Ti>
-__device__ float row_rinv(const AppendParams& p, const Ti* src, const Ti* w, int lane) {
-  if (w == nullptr) return 1.f;
+__device__ RowNorm norm_of_row(const AppendParams& p, const Ti* src, const Ti* w, int lane) {
+  if (w == nullptr) return {1.f, 1.f, true};
   float ss = 0.f;
   for (int d = lane; d < p.head_dim; d += 32) {
     const float x = to_f32(src[d]);
@@ -445,7 +466,7 @@ __device__ float row_rinv(const AppendParams& p, const Ti* src, const Ti* w, int
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  return 1.f / sqrtf(ss / static_cast<float>(p.head_dim) + p.eps);
+  return row_norm(ss / static_cast<float>(p.head_dim), p.eps);
 }
 
 template <typename Ti, typename To, bool k8>
@@ -465,9 +486,9 @@ __global__ void __launch_bounds__(kThreads) rope_append_generic_kernel(const App
       if (kind == 0) {
         const Ti* src = static_cast<const Ti*>(p.q_in) + t * p.q_in_stride + static_cast<int64_t>(i) * D;
         To* dst = static_cast<To*>(p.q_out) + t * p.q_out_stride + static_cast<int64_t>(i) * D;
-        const float rinv = row_rinv(p, src, qw, lane);
+        const RowNorm norm = norm_of_row(p, src, qw, lane);
         for (int d = lane; d < D; d += 32)
-          dst[d] = from_f32<To>(rotated_element(p, src, qw, rinv, pos, d));
+          dst[d] = from_f32<To>(rotated_element(p, src, qw, norm, pos, d));
         continue;
       }
       if (slot < 0) continue;
@@ -481,9 +502,9 @@ __global__ void __launch_bounds__(kThreads) rope_append_generic_kernel(const App
                 ((page * p.hkv + h) * S + (slot - page * S)) * D;
       if (kind == 1) {
         const Ti* src = static_cast<const Ti*>(p.k_in) + t * p.k_in_stride + static_cast<int64_t>(h) * D;
-        const float rinv = row_rinv(p, src, kw, lane);
+        const RowNorm norm = norm_of_row(p, src, kw, lane);
         for (int d = lane; d < D; d += 32)
-          dst[d] = from_f32<To>(rotated_element(p, src, kw, rinv, pos, d));
+          dst[d] = from_f32<To>(rotated_element(p, src, kw, norm, pos, d));
       } else {
         const Ti* src = static_cast<const Ti*>(p.v_in) + t * p.v_in_stride + static_cast<int64_t>(h) * D;
         for (int d = lane; d < D; d += 32) dst[d] = from_f32<To>(to_f32(src[d]));
@@ -510,14 +531,15 @@ __global__ void __launch_bounds__(kThreads) rope_append_generic_kernel(const App
         const int64_t block = page * p.hkv + h;
         uint8_t* tile = reinterpret_cast<uint8_t*>(is_v ? p.v_pool : p.k_pool) + block * S * D;
         float* scale = (is_v ? p.v_scale : p.k_scale) + block;
-        auto value = [&](int r, float rinv, int d) {
+        auto norm_at = [&](int r) { return norm_of_row(p, src + r * stride, is_v ? nullptr : kw, lane); };
+        auto value = [&](int r, const RowNorm& norm, int d) {
           const Ti* row = src + r * stride;
-          return is_v ? to_f32(row[d]) : rotated_element(p, row, kw, rinv, __ldg(p.positions + t + r), d);
+          return is_v ? to_f32(row[d]) : rotated_element(p, row, kw, norm, __ldg(p.positions + t + r), d);
         };
         float m = 0.f;
         for (int r = 0; r < n; ++r) {
-          const float rinv = is_v ? 1.f : row_rinv(p, src + r * stride, kw, lane);
-          for (int d = lane; d < D; d += 32) m = fmaxf(m, finite_abs(value(r, rinv, d)));
+          const RowNorm norm = norm_at(r);
+          for (int d = lane; d < D; d += 32) m = fmaxf(m, finite_abs(value(r, norm, d)));
         }
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -533,10 +555,10 @@ __global__ void __launch_bounds__(kThreads) rope_append_generic_kernel(const App
         if (lane == 0 && (off == 0 || old != s)) *scale = s;
         const float inv = exp2_int(-e);
         for (int r = 0; r < n; ++r) {
-          const float rinv = is_v ? 1.f : row_rinv(p, src + r * stride, kw, lane);
+          const RowNorm norm = norm_at(r);
           for (int d = lane; d < D; d += 32)
             tile[(off + r) * D + d] = static_cast<uint8_t>(
-                __nv_cvt_float_to_fp8(value(r, rinv, d) * inv, __NV_SATFINITE, __NV_E4M3));
+                __nv_cvt_float_to_fp8(value(r, norm, d) * inv, __NV_SATFINITE, __NV_E4M3));
         }
       }
     }
