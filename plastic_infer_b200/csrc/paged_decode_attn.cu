@@ -1107,17 +1107,17 @@ inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255);
 // Workspace = [arrival counters | partial (m, l) | partial O]. The counter block has
 // a fixed size and position whatever the batch shape, so a launch of one shape can
 // never find partials of an earlier launch of another shape where its counters are:
-// zeroed once, it stays zero because every launch resets the counters it used.
+// zeroed once, it stays zero because every launch resets the counters it used. The
+// attention over 8-bit pools keeps the same block (kAttnCounterBytes).
 // The last 256 bytes of the block hold the grid-completion counter of the gather
 // variant (it also returns to zero at the end of every launch).
-constexpr size_t kSegCounterBytes = static_cast<size_t>(kMaxBatch) * kMaxKvHeads * sizeof(int);
-constexpr size_t kCounterBytes = kSegCounterBytes + 256;
+static_assert(kMaxBatch * kMaxKvHeads <= kAttnSegments, "a counter for every segment");
 
 Layout ws_layout(int head_dim, int sms) {
   Layout L;
   const size_t slots = static_cast<size_t>(sms) * kMaxCtasPerSm * kWarps * 2;
   L.cnt_off = 0;
-  L.ml_off = align256(kCounterBytes);
+  L.ml_off = align256(kAttnCounterBytes);
   L.o_off = L.ml_off + align256(slots * kHeadsPad * 2 * sizeof(float));
   L.total = L.o_off + align256(slots * kHeadsPad * static_cast<size_t>(head_dim) * sizeof(float));
   return L;
@@ -1225,7 +1225,7 @@ extern "C" size_t pi_paged_decode_attn_workspace_bytes(int batch, int num_q_head
 }
 
 extern "C" size_t pi_paged_decode_attn_ws_zero_bytes(void) {
-  return pi::attn::align256(pi::attn::kCounterBytes);
+  return pi::attn::align256(pi::kAttnCounterBytes);
 }
 
 namespace pi {
@@ -1315,7 +1315,7 @@ int attn_dispatch(void* out, const void* q, const void* k_pool, const void* v_po
     fp.k_pool_w = const_cast<void*>(k_pool);
     fp.v_pool_w = const_cast<void*>(v_pool);
     fp.ag = {};
-    fp.ag_done = reinterpret_cast<unsigned*>(ws + L.cnt_off + kSegCounterBytes);
+    fp.ag_done = reinterpret_cast<unsigned*>(ws + L.cnt_off + kAttnSegmentBytes);
     if (ag != nullptr) {
       // The gather output rows are pushed as 16-byte chunks of whole row groups.
       if ((static_cast<int64_t>(group) * head_dim * eb) % 16 != 0 || (out_stride * eb) % 16 != 0 ||

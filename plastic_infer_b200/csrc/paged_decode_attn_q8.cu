@@ -56,7 +56,7 @@ constexpr int kWarps = 4;  // per CTA, each an independent consumer
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 32;            // tokens per step
 constexpr int kMaxBatch = 4096;
-constexpr int kMaxSegments = 4096 * 64;  // arrival counters
+constexpr int kMaxSegments = kAttnSegments;
 constexpr int kMaxCtasPerSm = 2;
 constexpr int kMaxTiles = 2;          // tiles of eight query rows per pass
 constexpr unsigned kFull = 0xffffffffu;
@@ -991,12 +991,12 @@ struct Layout {
 };
 inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 // [arrival counters | partial (max, sum) | partial O]; the counters have one place for every
-// shape, so zeroed once they stay zero between launches.
-constexpr size_t kCounterBytes = static_cast<size_t>(kMaxSegments) * sizeof(int);
+// shape, so zeroed once they stay zero between launches. The block is the 16-bit kernels' too, the
+// gather's completion counter at its end included: partials there would stop the next gather.
 Layout ws_layout(int head_dim, int sms) {
   Layout L;
   const size_t slots = static_cast<size_t>(sms) * kMaxCtasPerSm * kWarps * 2;
-  L.ml_off = align256(kCounterBytes);
+  L.ml_off = align256(kAttnCounterBytes);
   L.o_off = L.ml_off + align256(slots * 8 * kMaxTiles * 2 * sizeof(float));
   L.total = L.o_off + align256(slots * 8 * kMaxTiles * static_cast<size_t>(head_dim) * sizeof(float));
   return L;
@@ -1082,7 +1082,7 @@ extern "C" size_t pi_paged_decode_attn_q8_workspace_bytes(int head_dim) {
 }
 
 extern "C" size_t pi_paged_decode_attn_q8_ws_zero_bytes(void) {
-  return pi::q8::align256(pi::q8::kCounterBytes);
+  return pi::q8::align256(pi::kAttnCounterBytes);
 }
 
 extern "C" int pi_paged_decode_attn_q8(void* out, const void* q, const void* k_pool,

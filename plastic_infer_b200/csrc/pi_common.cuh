@@ -72,6 +72,13 @@ cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t 
   return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
 }
 
+// Every decode-attention workspace begins with the same zeroed block, so that calls over 16-bit and
+// 8-bit pools can share one: arrival counters of up to kAttnSegments (request, KV head) segments, then
+// 256 bytes that hold the peer gather's completion counter. Partial results lie behind the block.
+constexpr int kAttnSegments = 4096 * 64;
+constexpr size_t kAttnSegmentBytes = static_cast<size_t>(kAttnSegments) * sizeof(int);
+constexpr size_t kAttnCounterBytes = kAttnSegmentBytes + 256;
+
 // ---------------------------------------------------------------------------
 // Device-side error word: kernels never trap; they record the first error code
 // in an optional int the caller owns and skip the offending access.

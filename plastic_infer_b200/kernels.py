@@ -477,10 +477,12 @@ def expert_slot_copy(
 
 
 class Workspace:
-    """Zero-initialised device scratch for pi_paged_decode_attn, grown on demand.
+    """Zero-initialised device scratch for the paged attention calls, grown on demand.
 
-    The kernel leaves its counter region zero on exit, so the buffer is zeroed once
-    at allocation. Launches that share one Workspace must be ordered (same stream);
+    The kernels leave the counter region zero on exit, so the buffer is zeroed once
+    at allocation. paged_decode_attention, its gather variant and the 8-bit attention
+    calls may share one; host_stream_attention keeps no zeroed region and needs one of
+    its own. Launches that share one Workspace must be ordered (same stream);
     give concurrent streams their own Workspace.
     """
 

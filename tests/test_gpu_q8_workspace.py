@@ -1,0 +1,52 @@
+"""Scratch of the 8-bit attention calls: shared with the 16-bit ones, between streams and threads,
+grown and given back."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from plastic_infer_b200 import _capi, kernels
+from tests._q8 import DEV, cache, check, on_gpu, reference
+
+pytestmark = pytest.mark.gpu
+
+
+def queries(B, Hq, D, dtype, seed):
+    g = torch.Generator().manual_seed(seed + 300)
+    return torch.randn((B, Hq, D), generator=g).to(dtype).to(DEV)
+
+
+def decode(q, c, **kw):
+    return kernels.paged_decode_attention_q8(q, c["k_pool"], c["v_pool"], c["k_scale"], c["v_scale"],
+                                             c["tables"], c["lens"], **kw)
+
+
+def prefill(q, c, kv_len, q_start, **kw):
+    return kernels.paged_prefill_attention_q8(q, c["k_pool"], c["v_pool"], c["k_scale"], c["v_scale"],
+                                              c["tables"][0], kv_len, q_start, **kw)
+
+
+def counters(ws):
+    return ws.buf[:int(_capi.load().pi_paged_decode_attn_ws_zero_bytes())]
+
+
+@pytest.mark.parametrize("lens", [[4000], [900] * 40], ids=["merge launch", "last arriver"])
+def test_one_workspace_for_both_caches(lens):
+    # contexts cut across warps, so partial results are written; the block that the 16-bit kernels
+    # (the gather's completion counter at its end) need zeroed stays zero
+    c = on_gpu(cache(lens, 8, 128, 16, seed=50))
+    q = queries(len(lens), 32, 128, torch.bfloat16, 50)
+    ref, tol = reference(q, c, lens)
+    ws = kernels.Workspace(DEV)
+    k16 = kernels.page_dequant(c["k_pool"], c["k_scale"], torch.arange(c["k_pool"].shape[0], dtype=torch.int32, device=DEV))
+    v16 = kernels.page_dequant(c["v_pool"], c["v_scale"], torch.arange(c["k_pool"].shape[0], dtype=torch.int32, device=DEV))
+    tables = torch.where(c["tables"] < 2 ** 29, c["tables"], 0)
+    alone = kernels.paged_decode_attention(q, k16, v16, tables, c["lens"], workspace=kernels.Workspace(DEV))
+    for _ in range(2):
+        check(decode(q, c, workspace=ws), ref, tol)
+        assert int(counters(ws).count_nonzero()) == 0
+        assert torch.equal(kernels.paged_decode_attention(q, k16, v16, tables, c["lens"], workspace=ws), alone)
+        assert int(counters(ws).count_nonzero()) == 0
+        check(prefill(q[:1], c, lens[0], lens[0] - 1, workspace=ws), *(x[:1] for x in (ref, tol)))
+        assert int(counters(ws).count_nonzero()) == 0

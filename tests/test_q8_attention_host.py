@@ -155,3 +155,10 @@ def test_prefill_c_entries_validate_before_launch():
     assert d(a, a, a, a, -1, 2, 128, 16, 8, 1, None, None) == _capi.PI_ERR_BAD_SHAPE
     assert d(a, None, a, a, 1, 2, 128, 16, 8, 1, None, None) == _capi.PI_ERR_NULL_POINTER
     assert d(a, a, ctypes.c_void_p(257), a, 1, 2, 128, 16, 8, 1, None, None) == _capi.PI_ERR_MISALIGNED
+
+
+def test_one_zeroed_block_for_every_decode_attention():
+    # 16-bit and 8-bit calls may share a workspace: what either needs zeroed, neither writes over
+    _build.build()
+    lib = _capi.load()
+    assert lib.pi_paged_decode_attn_q8_ws_zero_bytes() == lib.pi_paged_decode_attn_ws_zero_bytes()
