@@ -255,8 +255,10 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const AppendParam
   const bool il = p.interleaved != 0;
   float2* table = reinterpret_cast<float2*>(smem);  // [tile (+ S - 1)][pairs]
   const int g = blockIdx.y, ng = p.groups;
-  const int q0 = p.hq * g / ng, q1 = p.hq * (g + 1) / ng;
-  const int h0 = p.hkv * g / ng, h1 = p.hkv * (g + 1) / ng;
+  // group i's first head: n / ng heads each, one more for the first n % ng (n * i may pass 32 bits)
+  auto first = [&](int n, int i) { return n / ng * i + min(i, n % ng); };
+  const int q0 = first(p.hq, g), q1 = first(p.hq, g + 1);
+  const int h0 = first(p.hkv, g), h1 = first(p.hkv, g + 1);
   __shared__ int64_t s_slot[k8 ? 64 + 32 : 1];
   __shared__ float s_max[2][kThreads / 32];
   // Where a token's K and V rows go (elements from the pools' start, head 0), -1: nowhere. Worked out
@@ -313,7 +315,9 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const AppendParam
                       : static_cast<const Ti*>(p.v_in) + tok * p.v_in_stride + h * D;
       const int64_t at = s_dst[k8 ? 0 : t];
       write = live && at >= 0;
-      dst = reinterpret_cast<To*>(kind == 1 ? p.k_pool : p.v_pool) + at + h * (p.page_size * D);
+      // (64 bits: a page of many tokens and heads may hold more than 2^31 elements)
+      dst = reinterpret_cast<To*>(kind == 1 ? p.k_pool : p.v_pool) + at +
+            h * (static_cast<int64_t>(p.page_size) * D);
     }
     float x[16];
 #pragma unroll
