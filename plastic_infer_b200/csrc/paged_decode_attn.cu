@@ -1036,7 +1036,8 @@ __global__ void __launch_bounds__(128) paged_decode_attn_simt_kernel(const SimtP
 // Host side: tensor-map cache, launch configuration, workspace layout.
 // ---------------------------------------------------------------------------------
 
-PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                  const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -1048,7 +1049,20 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
     }
   });
-  return fn;
+  if (!fn) return false;
+  const cuuint32_t ones[5] = {1u, 1u, 1u, 1u, 1u};
+  const auto encode = [&] {
+    return fn(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, ones,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  const CUresult r = encode();
+  if (r != CUDA_ERROR_INVALID_CONTEXT) return r == CUDA_SUCCESS;
+  // The driver needs a current context, and a host thread that makes its first CUDA call here has
+  // none yet: the runtime binds the device's own to it.
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+  return encode() == CUDA_SUCCESS;
 }
 
 struct MapKey {
@@ -1078,19 +1092,13 @@ bool pool_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, int D, i
       return true;
     }
   }
-  auto encode = get_encode();
-  if (!encode) return false;
   CUtensorMap m;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(D) * 2};
   cuuint32_t box[2] = {64u, static_cast<cuuint32_t>(S)};
-  cuuint32_t estr[2] = {1u, 1u};
   const CUtensorMapDataType dt =
       dtype == PI_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const CUresult r = encode(&m, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return false;
+  if (!encode_tiled(&m, dt, 2, base, dims, strides, box)) return false;
   const int slot = used < kCache ? used++ : (next++ % kCache);
   keys[slot] = key;
   maps[slot] = m;

@@ -47,7 +47,9 @@
 
 namespace pi {
 namespace attn {
-PFN_cuTensorMapEncodeTiled_v12000 get_encode();  // paged_decode_attn.cu
+// paged_decode_attn.cu
+bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                  const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
 }  // namespace attn
 
 namespace q8 {
@@ -975,15 +977,10 @@ __global__ void __launch_bounds__(128)
 
 // A pool as rows of 128 bytes; a page tile is one box.
 bool pool_map(CUtensorMap* m, const void* base, uint64_t rows, int box_rows) {
-  auto encode = attn::get_encode();
-  if (!encode) return false;
   cuuint64_t dims[2] = {128, rows};
   cuuint64_t strides[1] = {128};
   cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
-  cuuint32_t estr[2] = {1, 1};
-  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return attn::encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box);
 }
 
 struct Layout {

@@ -46,7 +46,8 @@ namespace attn {
 // Cached 2-D tensor map over a physical pool [rows = P*Hkv*S, D], and the driver's tensor-map
 // encoder (paged_decode_attn.cu).
 bool pool_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, int D, int S, int dtype);
-PFN_cuTensorMapEncodeTiled_v12000 get_encode();
+bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                  const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
 }  // namespace attn
 
 namespace prefill_tc {
@@ -638,18 +639,13 @@ bool configured[64][8] = {};
 // tensor read zeros, stores outside it are dropped.
 bool token_tensor_map(CUtensorMap* m, const void* base, int tokens, int heads, int D,
                       int64_t tok_stride, int G, int box_tokens, int dtype) {
-  auto encode = attn::get_encode();
-  if (!encode) return false;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads),
                         static_cast<cuuint64_t>(tokens)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(tok_stride) * 2};
   cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(box_tokens)};
-  cuuint32_t estr[3] = {1u, 1u, 1u};
   const CUtensorMapDataType dt =
       dtype == PI_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return encode(m, dt, 3, const_cast<void*>(base), dims, strides, box, estr,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return attn::encode_tiled(m, dt, 3, base, dims, strides, box);
 }
 
 template <typename T, int D, int S>
