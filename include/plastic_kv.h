@@ -489,7 +489,9 @@ int pi_rope_append(void* q_out, int64_t q_out_stride, void* k_pool, void* v_pool
  *   workspace      pi_paged_decode_attn_q8_workspace_bytes(head_dim) bytes, 256-byte aligned,
  *                  whose first pi_paged_decode_attn_q8_ws_zero_bytes() are zero before the first
  *                  call; every call leaves them zero (after PI_ERR_TIMEOUT in `err`, zero them
- *                  again). Calls that share one must be ordered. NULL is accepted where
+ *                  again). A call may be two launches that hand results over through it, so
+ *                  calls that share one must be ordered whole: same stream, and no other
+ *                  thread's call between a call's launches. NULL is accepted where
  *                  the generic kernel runs: f32, head sizes other than 64, 128 and 256, pages
  *                  other than 16 and 32.
  * head_dim <= 256. A page id outside the pool is reported through `err`, and the outputs of
@@ -520,7 +522,8 @@ int pi_paged_decode_attn_q8(void* out, const void* q, const void* k_pool, const 
  * power-of-two scales; an f16 value past 65504 becomes 65504) and pi_paged_prefill_attn_tc runs
  * on them; few, or shapes that it does not take: the kernels of pi_paged_decode_attn_q8.
  *   workspace   pi_paged_prefill_attn_q8_workspace_bytes(...) bytes; it begins with the
- *               scratch of pi_paged_decode_attn_q8, whose zeroed part is as there
+ *               scratch of pi_paged_decode_attn_q8, whose zeroed part is as there, and so is
+ *               the rule for calls that share one
  */
 size_t pi_paged_prefill_attn_q8_workspace_bytes(int q_len, int kv_len, int num_q_heads,
                                                 int num_kv_heads, int head_dim, int page_size,

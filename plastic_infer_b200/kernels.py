@@ -483,18 +483,23 @@ class Workspace:
     at allocation. paged_decode_attention, its gather variant and the 8-bit attention
     calls may share one; host_stream_attention keeps no zeroed region and needs one of
     its own. Launches that share one Workspace must be ordered (same stream);
-    give concurrent streams their own Workspace.
+    give concurrent streams their own Workspace. Threads may share one on one stream:
+    a call of several launches (the 8-bit attention) holds `lock` from get() until its
+    last launch is enqueued, so no other thread's launch comes between them.
     """
 
     def __init__(self, device: torch.device) -> None:
         self.device = torch.device(device)
         self.buf: torch.Tensor | None = None
+        self.lock = threading.RLock()
 
     def get(self, nbytes: int) -> torch.Tensor:
-        if self.buf is None or self.buf.numel() < nbytes:
-            n = max(nbytes, 1 << 20)
-            self.buf = torch.zeros(n, dtype=torch.uint8, device=self.device)
-        return self.buf
+        with self.lock:
+            buf = self.buf
+            if buf is None or buf.numel() < nbytes:
+                n = max(nbytes, 1 << 20)
+                self.buf = buf = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            return buf
 
 
 _ws_lock = threading.Lock()
@@ -663,24 +668,29 @@ def _check_q8_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.T
     return P, Hkv, S, D
 
 
-def _q8_workspace(device: torch.device, nbytes: int, workspace: Workspace | None) -> torch.Tensor:
-    """Scratch for one q8 attention call on the device's current stream: the caller's, or one
-    of the stream's own, so that calls on two streams never share it. Under graph capture it
-    comes out of the graph's memory, zeroed by the graph: no two graphs share it either."""
-    if workspace is not None:
-        if torch.device(workspace.device).index not in (None, device.index):
-            raise ValueError(f"the workspace is on {workspace.device}, q on {device}")
-        return workspace.get(nbytes)
-    if torch.cuda.is_current_stream_capturing():
+def _q8_call(device: torch.device, nbytes: int, workspace: Workspace | None,
+             err: torch.Tensor | None, func: str, *args) -> None:
+    """One q8 attention call on the device's current stream, with `nbytes` of scratch: the
+    caller's, or one of the stream's own, so that calls on two streams never share it. A call
+    may be several launches that hand data over through the scratch, so it is held against
+    other threads until all are enqueued. Under graph capture it comes out of the graph's
+    memory, zeroed by the graph: no two graphs share it either."""
+    if workspace is None and torch.cuda.is_current_stream_capturing():
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         buf[:int(_capi.load().pi_paged_decode_attn_q8_ws_zero_bytes())].zero_()
-        return buf
-    stream = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
-    ws = _q8_ws.get(stream)
-    if ws is None:
-        with _ws_lock:
-            ws = _q8_ws.setdefault(stream, Workspace(device))
-    return ws.get(nbytes)
+        _call_on(device, func, *args, buf.data_ptr(), nbytes, _err_ptr(err))
+        return
+    if workspace is None:
+        stream = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
+        workspace = _q8_ws.get(stream)
+        if workspace is None:
+            with _ws_lock:
+                workspace = _q8_ws.setdefault(stream, Workspace(device))
+    elif torch.device(workspace.device).index not in (None, device.index):
+        raise ValueError(f"the workspace is on {workspace.device}, q on {device}")
+    with workspace.lock:
+        buf = workspace.get(nbytes)
+        _call_on(device, func, *args, buf.data_ptr(), buf.numel(), _err_ptr(err))
 
 
 def _q8_decode_workspace_bytes(device: torch.device, head_dim: int) -> int:
@@ -714,7 +724,8 @@ def paged_decode_attention_q8(
     (bf16, f16 or f32); a request with no context gets zeros. What lies behind a request's last
     token is not used, whatever it holds. Head sizes 64, 128 and 256 with pages of 16 or 32 run
     on the tensor cores in bf16 and f16; everything else (head_dim <= 256) on a plain kernel.
-    Without `workspace`, calls on different streams and captured graphs have scratch of their own.
+    Without `workspace`, calls on different streams and captured graphs have scratch of their own;
+    threads that call on one stream, with or without one, do not disturb each other.
     """
     P, Hkv, S, D = _check_q8_pools(k_pool, v_pool, k_scale, v_scale)
     if q.dim() != 3 or q.shape[2] != D:
@@ -741,15 +752,13 @@ def paged_decode_attention_q8(
         return out
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    ws = _q8_workspace(device, _q8_decode_workspace_bytes(device, D), workspace)
     row = Hq * D
-    _call_on(
-        device, "pi_paged_decode_attn_q8",
+    _q8_call(
+        device, _q8_decode_workspace_bytes(device, D), workspace, err, "pi_paged_decode_attn_q8",
         out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
         v_scale.data_ptr(), block_tables.data_ptr(), block_tables.stride(0) if B > 1 else 0,
         block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv, D, S, P, float(scale), code,
-        q.stride(0) if B > 1 else row, out.stride(0) if B > 1 else row, ws.data_ptr(), ws.numel(),
-        _err_ptr(err),
+        q.stride(0) if B > 1 else row, out.stride(0) if B > 1 else row,
     )
     return out
 
@@ -812,15 +821,13 @@ def paged_prefill_attention_q8(
             with torch.cuda.device(device):
                 nbytes = int(_capi.load().pi_paged_prefill_attn_q8_workspace_bytes(
                     n, kv_len, Hq, Hkv, D, S, code))
-        ws = _q8_workspace(device, nbytes, workspace)
         row = Hq * D
-        _call_on(
-            device, "pi_paged_prefill_attn_q8",
+        _q8_call(
+            device, nbytes, workspace, err, "pi_paged_prefill_attn_q8",
             out3.data_ptr(), q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), block_table.numel(), n,
             kv_len, q_start, 1 if causal else 0, Hq, Hkv, D, S, P, float(scale), code,
-            q3.stride(0) if n > 1 else row, out3.stride(0) if n > 1 else row, ws.data_ptr(),
-            ws.numel(), _err_ptr(err),
+            q3.stride(0) if n > 1 else row, out3.stride(0) if n > 1 else row,
         )
     if out is not None:
         return out

@@ -3,6 +3,8 @@ grown and given back."""
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -50,3 +52,53 @@ def test_one_workspace_for_both_caches(lens):
         assert int(counters(ws).count_nonzero()) == 0
         check(prefill(q[:1], c, lens[0], lens[0] - 1, workspace=ws), *(x[:1] for x in (ref, tol)))
         assert int(counters(ws).count_nonzero()) == 0
+
+
+def run_threads(jobs, rounds):
+    """Every job in a thread of its own, on one stream, `rounds` times; the outputs by job."""
+    outs = [[] for _ in jobs]
+    failed = []
+    go = threading.Barrier(len(jobs))
+
+    def work(i):
+        try:
+            go.wait()
+            for _ in range(rounds):
+                outs[i].append(jobs[i]())
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    return outs
+
+
+@pytest.mark.parametrize("own", [False, True], ids=["hidden", "workspace"])
+def test_threads_on_one_stream(own):
+    # few segments: a launch that writes partial results and one that merges them; another thread's
+    # launches must not come between the two
+    ws = kernels.Workspace(DEV) if own else None
+    caches = [on_gpu(cache([n], 2, 128, 16, seed=60 + i)) for i, n in enumerate((3000, 2500, 1700))]
+    qs = [queries(1, 8, 128, torch.bfloat16, 60 + i) for i in range(3)]
+    want = [decode(q, c).clone() for q, c in zip(qs, caches)]
+    jobs = [lambda q=q, c=c: decode(q, c, workspace=ws) for q, c in zip(qs, caches)]
+    for w, got in zip(want, run_threads(jobs, 300)):
+        for o in got:
+            assert torch.equal(o, w)
+
+
+def test_threads_with_long_chunks():
+    # widened pages of one request must not be read by another's queries
+    lens = (1200, 700, 950)
+    caches = [on_gpu(cache([n], 4, 128, 16, seed=70 + i)) for i, n in enumerate(lens)]
+    qs = [queries(n // 2, 16, 128, torch.bfloat16, 70 + i) for i, n in enumerate(lens)]
+    want = [prefill(q, c, n, n - n // 2).clone() for q, c, n in zip(qs, caches, lens)]
+    jobs = [lambda q=q, c=c, n=n: prefill(q, c, n, n - n // 2) for q, c, n in zip(qs, caches, lens)]
+    for w, got in zip(want, run_threads(jobs, 60)):
+        for o in got:
+            assert torch.equal(o, w)

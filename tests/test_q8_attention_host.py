@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import threading
+import time
 
 import pytest
 import torch
@@ -162,3 +164,54 @@ def test_one_zeroed_block_for_every_decode_attention():
     _build.build()
     lib = _capi.load()
     assert lib.pi_paged_decode_attn_q8_ws_zero_bytes() == lib.pi_paged_decode_attn_ws_zero_bytes()
+
+
+@pytest.mark.parametrize("hidden", [False, True], ids=["workspace", "hidden"])
+def test_a_call_is_not_split_by_another_thread(monkeypatch, hidden):
+    # a call is several launches over one scratch: while one thread is in it, another with the same
+    # stream and scratch has to wait (the C call releases the interpreter lock)
+    ws = kernels.Workspace(torch.device("cpu"))
+    monkeypatch.setattr(kernels, "_check_one_device", lambda *t: torch.device("cuda", 0))
+    monkeypatch.setattr(kernels, "_q8_decode_workspace_bytes", lambda *a: 4096)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 7, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setitem(kernels._q8_ws, (0, 7), ws)
+    inside, most, done = [0], [0], []
+
+    def call_on(device, func, *args):
+        inside[0] += 1
+        most[0] = max(most[0], inside[0])
+        time.sleep(0.1)
+        inside[0] -= 1
+        done.append(func)
+
+    monkeypatch.setattr(kernels, "_call_on", call_on)
+
+    def work():
+        a = _args()
+        kernels.paged_decode_attention_q8(**a, out=torch.empty_like(a["q"]), workspace=None if hidden else ws)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(done) == 3 and most[0] == 1
+
+
+def test_workspace_gives_what_was_asked_for(monkeypatch):
+    # a thread that finds the buffer large enough gets it, whatever another does meanwhile
+    ws = kernels.Workspace(torch.device("cpu"))
+    short = []
+
+    def work(n):
+        for _ in range(200):
+            if ws.get(n).numel() < n:
+                short.append(n)
+
+    threads = [threading.Thread(target=work, args=((1 << 20) + 4096 * i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not short
