@@ -523,7 +523,8 @@ int pi_paged_decode_attn_q8(void* out, const void* q, const void* k_pool, const 
  * on them; few, or shapes that it does not take: the kernels of pi_paged_decode_attn_q8.
  *   workspace   pi_paged_prefill_attn_q8_workspace_bytes(...) bytes; it begins with the
  *               scratch of pi_paged_decode_attn_q8, whose zeroed part is as there, and so is
- *               the rule for calls that share one
+ *               the rule for calls that share one. Where these bytes are more than
+ *               pi_paged_decode_attn_q8_workspace_bytes(head_dim) it need not be zeroed
  */
 size_t pi_paged_prefill_attn_q8_workspace_bytes(int q_len, int kv_len, int num_q_heads,
                                                 int num_kv_heads, int head_dim, int page_size,

@@ -1380,6 +1380,11 @@ extern "C" int pi_paged_prefill_attn_q8(void* out, const void* q, const void* k_
     p.per_pass = per_pass;
     const int rc = q8::place(p, head_dim, workspace, workspace_bytes);
     if (rc != PI_OK) return rc;
+    // A workspace for widened pages is lent for the call, and not zeroed by its lender; rows that are
+    // not aligned for the tcgen05 kernel come here all the same.
+    if (q8::widens(q_len, kv_len, num_q_heads, num_kv_heads, head_dim, page_size, dtype) &&
+        cudaMemsetAsync(workspace, 0, kAttnCounterBytes, stream) != cudaSuccess)
+      return PI_ERR_CUDA;
     return dtype == PI_DTYPE_BF16 ? q8::launch_chunk<__nv_bfloat16>(p, k_pool, v_pool, head_dim, page_size, stream)
                                   : q8::launch_chunk<__half>(p, k_pool, v_pool, head_dim, page_size, stream);
   }

@@ -668,18 +668,27 @@ def _check_q8_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.T
     return P, Hkv, S, D
 
 
-def _q8_call(device: torch.device, nbytes: int, workspace: Workspace | None,
+def _q8_call(device: torch.device, head_dim: int, nbytes: int, workspace: Workspace | None,
              err: torch.Tensor | None, func: str, *args) -> None:
     """One q8 attention call on the device's current stream, with `nbytes` of scratch: the
     caller's, or one of the stream's own, so that calls on two streams never share it. A call
     may be several launches that hand data over through the scratch, so it is held against
     other threads until all are enqueued. Under graph capture it comes out of the graph's
-    memory, zeroed by the graph: no two graphs share it either."""
-    if workspace is None and torch.cuda.is_current_stream_capturing():
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        buf[:int(_capi.load().pi_paged_decode_attn_q8_ws_zero_bytes())].zero_()
-        _call_on(device, func, *args, buf.data_ptr(), nbytes, _err_ptr(err))
-        return
+    memory, zeroed by the graph: no two graphs share it either.
+
+    Scratch for widened pages (nbytes past the decode kernels') grows with the history, so it is
+    not kept: torch's allocator lends it for the call, in powers of two, that a prompt taken in
+    chunks leaves a few blocks behind and not one per chunk. It need not be zeroed."""
+    if workspace is None:
+        lent = nbytes > _q8_decode_workspace_bytes(device, head_dim)
+        capturing = torch.cuda.is_current_stream_capturing()
+        if lent or capturing:
+            size = nbytes if capturing else 1 << (nbytes - 1).bit_length()
+            buf = torch.empty(size, dtype=torch.uint8, device=device)
+            if not lent:
+                buf[:int(_capi.load().pi_paged_decode_attn_q8_ws_zero_bytes())].zero_()
+            _call_on(device, func, *args, buf.data_ptr(), size, _err_ptr(err))
+            return
     if workspace is None:
         stream = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
         workspace = _q8_ws.get(stream)
@@ -754,7 +763,7 @@ def paged_decode_attention_q8(
         scale = 1.0 / math.sqrt(D)
     row = Hq * D
     _q8_call(
-        device, _q8_decode_workspace_bytes(device, D), workspace, err, "pi_paged_decode_attn_q8",
+        device, D, _q8_decode_workspace_bytes(device, D), workspace, err, "pi_paged_decode_attn_q8",
         out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
         v_scale.data_ptr(), block_tables.data_ptr(), block_tables.stride(0) if B > 1 else 0,
         block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv, D, S, P, float(scale), code,
@@ -784,7 +793,8 @@ def paged_prefill_attention_q8(
     Query i sits at position q_start + i; with `causal` it sees keys j <= q_start + i. Returns
     [q_len, Hq, D] in q's dtype (the input's leading batch axis is kept when given). Long chunks
     widen the request's pages once into the workspace and run the tcgen05 prefill on them; short
-    ones, and shapes that it does not take, run the 8-bit decode kernels over several rows.
+    ones, and shapes that it does not take, run the 8-bit decode kernels over several rows. Without
+    `workspace` the widened pages are lent by torch's allocator for the call.
     """
     P, Hkv, S, D = _check_q8_pools(k_pool, v_pool, k_scale, v_scale)
     batched = q.dim() == 4
@@ -823,7 +833,7 @@ def paged_prefill_attention_q8(
                     n, kv_len, Hq, Hkv, D, S, code))
         row = Hq * D
         _q8_call(
-            device, nbytes, workspace, err, "pi_paged_prefill_attn_q8",
+            device, D, nbytes, workspace, err, "pi_paged_prefill_attn_q8",
             out3.data_ptr(), q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), block_table.numel(), n,
             kv_len, q_start, 1 if causal else 0, Hq, Hkv, D, S, P, float(scale), code,

@@ -102,3 +102,41 @@ def test_threads_with_long_chunks():
     for w, got in zip(want, run_threads(jobs, 60)):
         for o in got:
             assert torch.equal(o, w)
+
+
+def test_widened_pages_are_given_back():
+    # a prompt in growing chunks: nothing of the 16-bit copies stays allocated, and the allocator's
+    # blocks behind them are few
+    Hkv, D, S, chunk, n = 8, 128, 16, 512, 8192
+    c = on_gpu(cache([n], Hkv, D, S, seed=80))
+    q = queries(chunk, 32, D, torch.bfloat16, 80)
+    side = torch.cuda.Stream()  # a stream whose scratch is its own
+    with torch.cuda.stream(side):
+        prefill(q[:1], c, 1, 0)  # the decode kernels' scratch
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        before, reserved = torch.cuda.memory_allocated(), torch.cuda.memory_reserved()
+        out = torch.empty_like(q)
+        for end in range(chunk, n + 1, chunk):
+            prefill(q, c, end, end - chunk, out=out)
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() <= before + out.numel() * 2 + (1 << 20)
+        need = int(_capi.load().pi_paged_prefill_attn_q8_workspace_bytes(chunk, n, 32, Hkv, D, S, _capi.PI_DTYPE_BF16))
+        assert torch.cuda.memory_reserved() - reserved <= 4 * need + (16 << 20)
+    rows = list(range(0, chunk, 97))
+    ref, tol = reference(q[rows], c, [n - chunk + i + 1 for i in rows], rows_of=[0] * len(rows))
+    check(out[rows], ref, tol)
+
+
+def test_lent_scratch_need_not_be_zeroed():
+    # rows that are not 16-byte aligned keep to the decode kernels: many segments, whose counters lie
+    # in scratch that held something else before
+    Hkv, D, S, n = 4, 128, 16, 500
+    c = on_gpu(cache([n], Hkv, D, S, seed=81))
+    q = queries(420, 16 * D + 4, 1, torch.bfloat16, 81)[:, 4:, 0].unflatten(1, (16, D))
+    rows = list(range(0, 420, 41))
+    ref, tol = reference(q[rows], c, [n - 420 + i + 1 for i in rows], rows_of=[0] * len(rows))
+    for _ in range(2):
+        dirty = torch.full((64 << 20,), 0xA5, dtype=torch.uint8, device=DEV)
+        del dirty
+        check(prefill(q, c, n, n - 420)[rows], ref, tol)
