@@ -488,10 +488,11 @@ int pi_rope_append(void* q_out, int64_t q_out_stride, void* k_pool, void* v_pool
  *   block_tables   [batch, max_pages] int32, rows bt_stride elements apart (0: one table for all)
  *   workspace      pi_paged_decode_attn_q8_workspace_bytes(head_dim) bytes, 256-byte aligned,
  *                  whose first pi_paged_decode_attn_q8_ws_zero_bytes() are zero before the first
- *                  call; every call leaves them zero (after PI_ERR_TIMEOUT in `err`, zero them
- *                  again). A call may be two launches that hand results over through it, so
- *                  calls that share one must be ordered whole: same stream, and no other
- *                  thread's call between a call's launches. NULL is accepted where
+ *                  call; every call leaves them zero, one that reports PI_ERR_TIMEOUT in
+ *                  `err` (its outputs are unspecified) too. A call may be two launches that
+ *                  hand results over through it, so calls that share one must be ordered
+ *                  whole: same stream, and no other thread's call between a call's launches.
+ *                  NULL is accepted where
  *                  the generic kernel runs: f32, head sizes other than 64, 128 and 256, pages
  *                  other than 16 and 32.
  * head_dim <= 256. A page id outside the pool is reported through `err`, and the outputs of

@@ -44,6 +44,7 @@
 #include <cudaTypedefs.h>
 
 #include "pi_common.cuh"
+#include "q8_split.cuh"
 
 namespace pi {
 namespace attn {
@@ -266,10 +267,12 @@ __device__ __noinline__ void merge_pieces(const Rows<T> dst, const float* ml0, c
   }
 }
 
-// Warps that share a stream of `total` units.
-__device__ __forceinline__ int active_warps(int64_t total, int nw) {
-  const int64_t most = (total + 1) / 2;
-  return static_cast<int>(most < nw ? most : nw);
+// The arrivals of a warp whose wait expired (one lane; noinline: never on the way of a sound launch).
+__device__ __noinline__ void give_up(const Split& s, const int* uoff, int requests, int HV, int warp, int64_t pos,
+                                     int* counters) {
+  abandon(s, uoff, requests, HV, warp, pos, [&](int segment, int pieces) {
+    if (atomicAdd(counters + segment, 1) == pieces - 1) counters[segment] = 0;
+  });
 }
 
 // Few segments have many pieces each: one warp that merges 150 of them after the stream's end takes
@@ -304,12 +307,11 @@ __global__ void __launch_bounds__(128) merge_kernel(const Params p, int S, int N
   const int64_t total = static_cast<int64_t>(all) * HV;
   const int cn = s_units[b];
   if (cn == 0 || row >= n) return;
-  const int nwe = active_warps(total, NW);
+  const Split split{total, active_warps(total, NW)};
   const int64_t start = static_cast<int64_t>(before) * HV + static_cast<int64_t>(hv) * cn;
-  const int wa = static_cast<int>(((start + 1) * nwe - 1) / total);
-  const int wb = static_cast<int>(((start + cn) * nwe - 1) / total);
+  const int wa = split.owner(start), wb = split.owner(start + cn - 1);
   if (wa == wb) return;  // one warp had it all and has written it
-  const int role_a = total * wa / nwe == start ? 0 : 1;
+  const int role_a = split.first(wa) == start ? 0 : 1;
   const int np = wb - wa + 1;
   auto at = [&](int j) { return (static_cast<int64_t>(wa + j) * 2 + (j == 0 ? role_a : 0)) * kPad + row; };
   const float2* ml = reinterpret_cast<const float2*>(p.ws_ml);
@@ -424,13 +426,10 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
   const int NW = gridDim.x * kWarps;
   const int gw = blockIdx.x * kWarps + warp;
   const int64_t total = static_cast<int64_t>(s_uoff[B]) * HV;
-  // Every active warp owns at least one unit: a segment's pieces are the warps that overlap it. Two
-  // at least where there are enough: a piece more costs its merge more than a unit costs its warp
-  // (1000 tokens of 8 KV heads: 14.6 us against 16.5 with one unit per warp).
-  const int NWe = active_warps(total, NW);
-  const bool active = gw < NWe;
-  const int64_t lo = active ? total * gw / NWe : 0;
-  const int64_t hi = active ? total * (gw + 1) / NWe : 0;
+  const Split split{total, active_warps(total, NW)};  // a segment's pieces are the warps that overlap it
+  const bool active = gw < split.warps;
+  const int64_t lo = active ? split.first(gw) : 0;
+  const int64_t hi = active ? split.first(gw + 1) : 0;
 
   // (request, head pass, unit) of a stream position; positions fit 32 bits (fast_shape)
   auto locate = [&](int64_t pos64, int& b, int& hv, int& u) {
@@ -665,12 +664,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
     int old = 0;
     if (lane == 0) old = atomicAdd(cnt, 1);
     old = __shfl_sync(kFull, old, 0);
-    const int wa = static_cast<int>(((seg_start + 1) * NWe - 1) / total);
-    const int wb = static_cast<int>((seg_end * NWe - 1) / total);
-    const int npieces = wb - wa + 1;
+    const int wa = split.owner(seg_start);
+    const int npieces = split.owner(seg_end - 1) - wa + 1;
     if (old != npieces - 1) return;
     __threadfence();
-    const int role_a = (total * wa / NWe == seg_start) ? 0 : 1;
+    const int role_a = split.first(wa) == seg_start ? 0 : 1;
     merge_pieces<T, D, kPad>(rows, p.ws_ml, p.ws_o, wa, npieces, role_a, n, lane);
     if (lane == 0) *cnt = 0;
   };
@@ -868,6 +866,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
   if (failed) {  // loads in flight land before the shared memory is released
     for (int64_t j = k; j < issued - lo; ++j)
       mbar_wait_bounded(bar0 + 8 * static_cast<int>(j % NS), static_cast<uint32_t>((j / NS) & 1));
+    if (lane == 0 && !p.merge_later) give_up(split, s_uoff, B, HV, gw, pos, p.ws_cnt);
   }
 }
 
