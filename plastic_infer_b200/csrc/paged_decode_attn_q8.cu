@@ -536,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
   sc_cur = load_scales(id_cur);
   sc_nxt = load_scales(id_nxt);
   for (int s = 0; s < issued - lo; ++s) put_scales(lo + s, s);
+  __syncwarp();  // one lane each wrote them, every lane reads them
 
   const int gid = lane >> 2;
   const int tig = lane & 3;
