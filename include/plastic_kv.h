@@ -54,6 +54,8 @@ extern "C" {
 #define PI_ERR_PAGE_RANGE 8   /* device-side: page id outside the pool (zero read)  */
 #define PI_ERR_TIMEOUT 9      /* device-side: a bounded wait gave up                */
 #define PI_ERR_SCRATCH_LIMIT 10 /* request needs more than the built-in scratch     */
+#define PI_ERR_PAGE_SHARED 11 /* device-side: an 8-bit page named by several runs of
+                                 one pi_rope_append (none of them written)          */
 
 /* element types */
 #define PI_DTYPE_F32 0
@@ -461,8 +463,11 @@ int pi_decode_prologue(void* q_out, int64_t q_out_stride, void* k_pool, void* v_
  * amax over the run's finite values; kept rows are those at offsets below the run's first
  * (a run at offset 0 keeps none and starts the block anew), rescaled when e grows. Values
  * beyond +-448 * 2^e (infinities) saturate, NaN stays NaN, rows behind the run are left as
- * they were. At most one run per page and call: with several, or with a slot named twice,
- * which of their rows and scales a page ends up with is unspecified (nothing else is touched).
+ * they were. At most one run per page and call. Where several name a page (tokens out of
+ * order, a gap or padding between a page's tokens, a slot named twice) and `err` is given, none
+ * of them is written, the page and its scales stay as they were and `err` gets
+ * PI_ERR_PAGE_SHARED; without `err` nobody looks, and which of their rows and scales that page
+ * ends up with is unspecified. q_out and the other pages are written either way.
  */
 int pi_rope_append(void* q_out, int64_t q_out_stride, void* k_pool, void* v_pool, float* k_scale,
                    float* v_scale, const void* q_in, int64_t q_in_stride, const void* k_in,

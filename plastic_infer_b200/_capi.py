@@ -28,6 +28,7 @@ PI_ERR_SLOT_RANGE = 7
 PI_ERR_PAGE_RANGE = 8
 PI_ERR_TIMEOUT = 9
 PI_ERR_SCRATCH_LIMIT = 10
+PI_ERR_PAGE_SHARED = 11
 NOALLOC_SCRATCH_BYTES = 12 << 20  # PI_NOALLOC_SCRATCH_BYTES in include/plastic_kv.h
 
 PI_ATTN_RING_AUTO = 0

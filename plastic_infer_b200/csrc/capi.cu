@@ -59,6 +59,7 @@ extern "C" const char* pi_error_string(int code) {
     case PI_ERR_SCRATCH_LIMIT:
       return "request needs more scratch than the allocation-free entry point's built-in "
              "array (PI_NOALLOC_SCRATCH_BYTES); use pi_paged_decode_attn with a workspace";
+    case PI_ERR_PAGE_SHARED: return "an 8-bit page named by several runs of one call (write skipped)";
     default: return "unknown status code";
   }
 }

@@ -19,6 +19,11 @@
 // against amax / 448 (e4m3 is a floating format: the step relative to a value is the same) and
 // makes rescaling an exponent shift, exact above e4m3's subnormals; values times scale are
 // exact in bf16. A run at offset 0 starts the block anew. Rows behind the run keep their bytes.
+// A page takes one run per call: two would have to agree on its scale and its kept rows, and they
+// belong to CTAs that cannot wait for one another. Where there is an `err` to tell it by, the CTA of a
+// run counts the call's tokens that name its page, and where they are more than the run's, no run of
+// that page is written. That reads all slots in every such CTA (L2): 8192 tokens take 80 us so
+// and 75 without, 64 take 7.1 and 6.4 in a graph, which is why a call without `err` does not look.
 //
 // What bounds it: every byte is moved once, so HBM; for a step of 64 tokens, latency. A CTA
 // takes a tile of tokens and a group of heads, and computes the tile's cosines and sines once
@@ -236,6 +241,38 @@ __device__ __forceinline__ bool run_starts(const int64_t* slots, int i, int page
   return s >= 0 && !(slots[i] >= 0 && s == slots[i] + 1 && s % page_size != 0);
 }
 
+// Adds to named[i], for each token i of the tile that starts a run (a bit of `starts`), the call's tokens
+// whose page has the same low 32 bits. All threads call.
+template <int S>
+__device__ __noinline__ void count_named(const int64_t* slot_mapping, int64_t n, uint32_t starts, const int64_t* slots,
+                                         int* named, int tid) {
+  constexpr int kShift = S == 16 ? 4 : 5;
+  static_assert(S == 1 << kShift, "pages of 16 or 32 tokens");
+  constexpr int kBatch = 16;  // loads in flight
+  auto count = [&](const uint32_t* page, int batch) {
+    for (uint32_t left = starts; left != 0; left &= left - 1) {
+      const int i = __ffs(left) - 1;
+      const uint32_t own = static_cast<uint32_t>(slots[i + 1] >> kShift);
+      int c = 0;
+#pragma unroll
+      for (int e = 0; e < batch; ++e) c += page[e] == own ? 1 : 0;
+      if (c != 0) atomicAdd(named + i, c);
+    }
+  };
+  int64_t j = tid;
+  for (; j + (kBatch - 1) * kThreads < n; j += kBatch * kThreads) {
+    uint32_t page[kBatch];
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e)
+      page[e] = static_cast<uint32_t>(__ldg(slot_mapping + j + e * kThreads) >> kShift);
+    count(page, kBatch);
+  }
+  for (; j < n; j += kThreads) {
+    const uint32_t page = static_cast<uint32_t>(__ldg(slot_mapping + j) >> kShift);
+    count(&page, 1);
+  }
+}
+
 // kPoolBits 8: K and V rows go to e4m3 blocks (To is then q's output type); else To is the
 // pools' type too. S: page size (8-bit pools only).
 template <typename Ti, typename To, int D, bool k8, int S>
@@ -259,6 +296,7 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const AppendParam
   const int h0 = first(p.hkv, g), h1 = first(p.hkv, g + 1);
   __shared__ int64_t s_slot[k8 ? 64 + 32 : 1];
   __shared__ float s_max[2][kThreads / 32];
+  __shared__ int s_named[kMaxTile];  // 8-bit: tokens of the call that name the page of the run at a token
   // Where a token's K and V rows go (elements from the pools' start, head 0), -1: nowhere. Worked out
   // once per token: the 64-bit division per row cost more than moving it.
   __shared__ int64_t s_dst[k8 ? 1 : kMaxTile];
@@ -275,11 +313,17 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const AppendParam
   if constexpr (k8) {
     for (int i = tid; i <= ext; i += kThreads)
       s_slot[i] = t0 + i == 0 ? -1 : __ldg(p.slot_mapping + t0 + i - 1);
+    if (tid < kMaxTile) s_named[tid] = 0;
     __syncthreads();
     // the last run may go on behind the tile
     if (h1 > h0 && s_slot[nt] >= 0)
       while (covered < ext && s_slot[covered + 1] == s_slot[covered] + 1 && s_slot[covered + 1] % S != 0)
         ++covered;
+    if (p.err != nullptr && h1 > h0) {
+      uint32_t starts = 0;
+      for (int i = 0; i < nt; ++i) starts |= run_starts(s_slot, i, S) ? 1u << i : 0u;
+      if (starts != 0) count_named<S>(p.slot_mapping, p.n_tokens, starts, s_slot, s_named, tid);
+    }
   }
   for (int i = tid; i < covered * pairs; i += kThreads) {
     const int t = i / pairs;
@@ -356,6 +400,17 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const AppendParam
       const int off = static_cast<int>(slot - page * S);
       int n = 1;
       while (i + n < covered && off + n < S && s_slot[i + 1 + n] == slot + n) ++n;
+      if (p.err != nullptr && h1 > h0 && s_named[i] != n) {
+        // other tokens name the page, or slots far outside the pool whose pages are alike in 32 bits
+        bool other = false;
+        for (int64_t j = tid; j < p.n_tokens; j += kThreads)
+          other |= static_cast<uint64_t>(__ldg(p.slot_mapping + j) - (slot - off)) < S &&
+                   (j < t0 + i || j >= t0 + i + n);
+        if (__syncthreads_or(other)) {
+          if (tid == 0) record_error(p.err, PI_ERR_PAGE_SHARED);
+          continue;
+        }
+      }
       for (int h = h0; h < h1; ++h) {
         const int64_t block = page * p.hkv + h;
         float k[kPass][16], v[kPass][16];
@@ -524,6 +579,14 @@ __global__ void __launch_bounds__(kThreads) rope_append_generic_kernel(const App
       const int off = static_cast<int>(slot - page * S);
       int n = 1;
       while (t + n < p.n_tokens && off + n < S && __ldg(p.slot_mapping + t + n) == slot + n) ++n;
+      bool other = false;
+      for (int64_t j = threadIdx.x; p.err != nullptr && j < p.n_tokens; j += kThreads)
+        other |= static_cast<uint64_t>(__ldg(p.slot_mapping + j) - (slot - off)) < static_cast<uint64_t>(S) &&
+                 (j < t || j >= t + n);
+      if (__syncthreads_or(other)) {
+        if (threadIdx.x == 0) record_error(p.err, PI_ERR_PAGE_SHARED);
+        continue;
+      }
       for (int i = warp; i < 2 * p.hkv; i += nw) {
         const bool is_v = i >= p.hkv;
         const int h = is_v ? i - p.hkv : i;

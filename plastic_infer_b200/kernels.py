@@ -357,7 +357,10 @@ def rope_append(
     dtype): each (page, head) block has one power-of-two scale, grown as rows arrive; the rows
     of one call in one page must be consecutive tokens with consecutive slots, rows at lower
     offsets are kept (rescaled when the scale grows), rows behind are left as they were
-    (include/plastic_kv.h has the formulas).
+    (include/plastic_kv.h has the formulas). With `err`, a page named in any other way (out of
+    order, with gaps or padding between its tokens, a slot twice) is left as it was and `err`
+    gets PI_ERR_PAGE_SHARED; without, nobody looks, and what that page ends up with is
+    unspecified.
     """
     P, Hkv, S, D = _check_pool(k_pool, "k_pool")
     if v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype:
