@@ -874,8 +874,9 @@ def page_dequant(pool: torch.Tensor, scale: torch.Tensor, page_ids: torch.Tensor
     elif out.dtype != dtype or tuple(out.shape) != (n, Hkv, S, D) or not out.is_contiguous():
         raise ValueError(f"out must be contiguous [{n}, {Hkv}, {S}, {D}] {dtype}")
     if n:
+        page_ids = page_ids.contiguous()  # (kept until the launch is enqueued)
         _call_on(device, "pi_page_dequant", out.data_ptr(), pool.data_ptr(), scale.data_ptr(),
-                 page_ids.contiguous().data_ptr(), n, Hkv, D, S, P, code, _err_ptr(err))
+                 page_ids.data_ptr(), n, Hkv, D, S, P, code, _err_ptr(err))
     return out
 
 

@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 import threading
 import time
+import weakref
 
 import pytest
 import torch
@@ -215,3 +216,26 @@ def test_workspace_gives_what_was_asked_for(monkeypatch):
     for t in threads:
         t.join()
     assert not short
+
+
+def test_page_dequant_keeps_its_copy_of_the_ids(monkeypatch):
+    # strided ids are copied; the copy has to live until the launch is enqueued, or its memory may be
+    # another thread's by then
+    copies = []
+    real = torch.Tensor.contiguous
+
+    def contiguous(t, *a):
+        c = real(t, *a)
+        if c is not t:
+            copies.append(weakref.ref(c))
+        return c
+
+    def call_on(device, func, *args):
+        assert len(copies) == 1 and copies[0]() is not None and copies[0]().data_ptr() in args
+
+    monkeypatch.setattr(torch.Tensor, "contiguous", contiguous)
+    monkeypatch.setattr(kernels, "_check_one_device", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(kernels, "_call_on", call_on)
+    kernels.page_dequant(torch.zeros(4, 2, 16, 64).to(E4M3), torch.ones(4, 2),
+                         torch.zeros(6, dtype=torch.int32)[::2])
+    assert len(copies) == 1
