@@ -722,7 +722,8 @@ extern "C" int pi_rope_append(void* q_out, int64_t q_out_stride, void* k_pool, v
     return PI_ERR_MISALIGNED;
   const int out_bytes = k8 ? in_bytes : elem_bytes_of(pool_dtype);
   if (!aligned(q_in, in_bytes) || !aligned(k_in, in_bytes) || !aligned(v_in, in_bytes) ||
-      !aligned(q_out, out_bytes) || (!k8 && (!aligned(k_pool, out_bytes) || !aligned(v_pool, out_bytes))))
+      !aligned(q_norm_w, in_bytes) || !aligned(k_norm_w, in_bytes) || !aligned(q_out, out_bytes) ||
+      (!k8 && (!aligned(k_pool, out_bytes) || !aligned(v_pool, out_bytes))))
     return PI_ERR_MISALIGNED;
   AppendParams p;
   p.q_out = q_out;

@@ -122,3 +122,17 @@ def test_oracle_rounding_is_torchs():
                           x.float().to(torch.float8_e4m3fn).double().numpy())
     for top, e in ((448.0, 0), (448.1, 1), (1.75, -8), (1.7500001, -7), (0.0, -118), (1e-44, -118)):
         assert orc.block_exp(np.array([top, -0.1 * top])) == e
+
+
+def test_c_entry_refuses_misaligned_weights():
+    # an address that the type's loads would fault on
+    _build.build()
+    f = _capi.load().pi_rope_append
+    a = ctypes.c_void_p(256)
+    for dtype, size in ((_capi.PI_DTYPE_BF16, 2), (_capi.PI_DTYPE_F16, 2), (_capi.PI_DTYPE_F32, 4)):
+        for qw, kw in ((256 + size // 2, 256), (256, 256 + size // 2)):
+            args = [a, 256, a, a, None, None, a, 256, a, 128, a, 128, dtype, ctypes.c_void_p(qw), ctypes.c_void_p(kw),
+                    1e-5, a, 32, 0, 1.0, a, a, 0, 4, 2, 64, 16, 8, dtype, None, None]
+            assert f(*args) == _capi.PI_OK  # no tokens: nothing is looked at
+            args[22] = 4
+            assert f(*args) == _capi.PI_ERR_MISALIGNED
