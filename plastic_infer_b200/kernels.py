@@ -313,6 +313,11 @@ def _check_one_device(*tensors: torch.Tensor | None) -> torch.device:
     return device  # type: ignore[return-value]
 
 
+def _head_rows(t: torch.Tensor) -> bool:
+    """Whether t [n, heads, D] has contiguous heads (a single head's stride means nothing)."""
+    return t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == t.shape[2])
+
+
 def _call_on(device: torch.device, func: str, *args) -> None:
     """_capi.call on the current stream of `device`, with that device current."""
     stream = torch._C._cuda_getCurrentRawStream(device.index)
@@ -383,7 +388,7 @@ def rope_append(
     pool_code = _capi.PI_DTYPE_E4M3 if eight else dtype_code(k_pool.dtype)
     out_dtype = q.dtype if eight else k_pool.dtype
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.stride(2) != 1 or t.stride(1) != D:
+        if not _head_rows(t):
             raise ValueError(f"{name}: heads must be contiguous rows of head_dim elements")
     if positions.dtype != torch.int64 or positions.shape != (T,):
         raise ValueError("positions must be int64 [T]")
@@ -395,8 +400,7 @@ def rope_append(
         raise ValueError("give both QK-norm weights or neither")
     if q_out is None:
         q_out = torch.empty((T, Hq, D), dtype=out_dtype, device=q.device)
-    elif q_out.dtype != out_dtype or tuple(q_out.shape) != (T, Hq, D) or q_out.stride(2) != 1 \
-            or q_out.stride(1) != D:
+    elif q_out.dtype != out_dtype or tuple(q_out.shape) != (T, Hq, D) or not _head_rows(q_out):
         raise ValueError(f"q_out must be [T, Hq, D] {out_dtype} with contiguous heads")
     qw = kw = None
     if q_norm_weight is not None:
@@ -760,12 +764,12 @@ def paged_decode_attention_q8(
     if ctx_lens.dtype != torch.int32 or ctx_lens.shape != (B,):
         raise ValueError("ctx_lens must be int32 [B]")
     device = _check_one_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, ctx_lens, out, err)
-    if q.stride(2) != 1 or q.stride(1) != D or (B > 1 and q.stride(0) < Hq * D):
+    if not _head_rows(q) or (B > 1 and q.stride(0) < Hq * D):
         q = q.contiguous()
     block_tables, ctx_lens = _early_reads(block_tables, ctx_lens)
     if out is None:
         out = torch.empty((B, Hq, D), dtype=q.dtype, device=device)
-    elif out.shape != (B, Hq, D) or out.dtype != q.dtype or out.stride(2) != 1 or out.stride(1) != D:
+    elif out.shape != (B, Hq, D) or out.dtype != q.dtype or not _head_rows(out):
         raise ValueError("out must be [B, Hq, D] with contiguous heads, q's dtype")
     if B == 0:
         return out
@@ -823,15 +827,14 @@ def paged_prefill_attention_q8(
     if kv_len > block_table.numel() * S or kv_len < 0 or q_start < 0 or q_start + n > 2 ** 31 - 1:
         raise ValueError("kv_len must be within the block table's pages, q_start not negative")
     device = _check_one_device(q3, k_pool, v_pool, k_scale, v_scale, block_table, out, err)
-    if q3.stride(2) != 1 or q3.stride(1) != D or (n > 1 and q3.stride(0) < Hq * D):
+    if not _head_rows(q3) or (n > 1 and q3.stride(0) < Hq * D):
         q3 = q3.contiguous()
     block_table, = _early_reads(block_table)
     if out is None:
         out3 = torch.empty((n, Hq, D), dtype=q3.dtype, device=device)
     else:
         out3 = out[0] if out.dim() == 4 else out
-        if out3.shape != (n, Hq, D) or out3.dtype != q3.dtype or out3.stride(2) != 1 \
-                or out3.stride(1) != D:
+        if out3.shape != (n, Hq, D) or out3.dtype != q3.dtype or not _head_rows(out3):
             raise ValueError("out must be [q_len, Hq, D] in q's dtype with contiguous heads")
     if n > 0:
         if scale is None:

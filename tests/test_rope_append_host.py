@@ -136,3 +136,10 @@ def test_c_entry_refuses_misaligned_weights():
             assert f(*args) == _capi.PI_OK  # no tokens: nothing is looked at
             args[22] = 4
             assert f(*args) == _capi.PI_ERR_MISALIGNED
+
+
+def test_one_head_of_any_stride_is_taken():
+    # refused for the device alone: [1, T, D] transposed has a head stride of T * D
+    x = torch.zeros((1, 3, 64), dtype=torch.bfloat16).transpose(0, 1)
+    with pytest.raises(ValueError, match="CUDA"):
+        kernels.rope_append(**{**_args(Hq=1, Hkv=1), "q": x, "k": x, "v": x}, q_out=x.clone(memory_format=torch.preserve_format))
