@@ -565,12 +565,11 @@ def decode_attn_ring_stages(batch: int, bt_stride: int, num_q_heads: int, num_kv
         dtype_code(dtype)))
 
 
-def _early_reads(*tables: torch.Tensor, rows_apart: bool = True) -> list[torch.Tensor]:
-    """The block tables and lengths of an attention call with unit inner strides, contiguous
-    without `rows_apart`. The kernel reads them before it waits for the launch before it
-    (set_programmatic_launch), so where one had to be copied, another launch is put between the
-    copy and the kernel."""
-    dense = [t if rows_apart and t.stride(-1) == 1 else t.contiguous() for t in tables]
+def _early_reads(*tables: torch.Tensor) -> list[torch.Tensor]:
+    """Contiguous block tables and lengths of an attention call. The kernel reads them before it
+    waits for the launch before it (set_programmatic_launch), so where one had to be copied,
+    another launch is put between the copy and the kernel."""
+    dense = [t.contiguous() for t in tables]
     if any(d.data_ptr() != t.data_ptr() for d, t in zip(dense, tables)):
         torch.zeros(1, dtype=torch.int32, device=dense[0].device)
     return dense
@@ -620,7 +619,8 @@ def paged_decode_attention(
     _require_cuda(q, k_pool, v_pool, block_tables, ctx_lens)
     if q.stride(2) != 1 or q.stride(1) != D:
         q = q.contiguous()
-    block_tables, ctx_lens = _early_reads(block_tables, ctx_lens)
+    if block_tables.stride(1) != 1 or ctx_lens.stride(0) != 1:  # (rows may be apart)
+        block_tables, ctx_lens = _early_reads(block_tables, ctx_lens)
     if out is None:
         out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
     elif out.shape != (B, Hq, D) or out.dtype != q.dtype or out.stride(2) != 1 or out.stride(1) != D:
@@ -766,7 +766,8 @@ def paged_decode_attention_q8(
     device = _check_one_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, ctx_lens, out, err)
     if not _head_rows(q) or (B > 1 and q.stride(0) < Hq * D):
         q = q.contiguous()
-    block_tables, ctx_lens = _early_reads(block_tables, ctx_lens)
+    if block_tables.stride(1) != 1 or ctx_lens.stride(0) != 1:  # (rows may be apart)
+        block_tables, ctx_lens = _early_reads(block_tables, ctx_lens)
     if out is None:
         out = torch.empty((B, Hq, D), dtype=q.dtype, device=device)
     elif out.shape != (B, Hq, D) or out.dtype != q.dtype or not _head_rows(out):
@@ -829,7 +830,8 @@ def paged_prefill_attention_q8(
     device = _check_one_device(q3, k_pool, v_pool, k_scale, v_scale, block_table, out, err)
     if not _head_rows(q3) or (n > 1 and q3.stride(0) < Hq * D):
         q3 = q3.contiguous()
-    block_table, = _early_reads(block_table)
+    if block_table.stride(0) != 1:
+        block_table, = _early_reads(block_table)
     if out is None:
         out3 = torch.empty((n, Hq, D), dtype=q3.dtype, device=device)
     else:
@@ -1239,7 +1241,7 @@ def paged_decode_attention_gather(
         raise ValueError("exchange was built for another shape or dtype")
     _require_cuda(q, k_pool, v_pool, block_tables, ctx_lens)
     q = q.contiguous()
-    block_tables, ctx_lens = _early_reads(block_tables, ctx_lens, rows_apart=False)
+    block_tables, ctx_lens = _early_reads(block_tables, ctx_lens)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     ex = exchange
