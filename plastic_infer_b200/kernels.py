@@ -684,6 +684,14 @@ def _check_q8_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.T
     return P, Hkv, S, D
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the current stream of `device`, current or not, is being captured."""
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _q8_call(device: torch.device, head_dim: int, nbytes: int, workspace: Workspace | None,
              err: torch.Tensor | None, func: str, *args) -> None:
     """One q8 attention call on the device's current stream, with `nbytes` of scratch: the
@@ -697,7 +705,7 @@ def _q8_call(device: torch.device, head_dim: int, nbytes: int, workspace: Worksp
     chunks leaves a few blocks behind and not one per chunk. It need not be zeroed."""
     if workspace is None:
         lent = nbytes > _q8_decode_workspace_bytes(device, head_dim)
-        capturing = torch.cuda.is_current_stream_capturing()
+        capturing = _capturing(device)
         if lent or capturing:
             size = nbytes if capturing else 1 << (nbytes - 1).bit_length()
             buf = torch.empty(size, dtype=torch.uint8, device=device)

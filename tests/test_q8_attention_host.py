@@ -176,6 +176,7 @@ def test_a_call_is_not_split_by_another_thread(monkeypatch, hidden):
     monkeypatch.setattr(kernels, "_q8_decode_workspace_bytes", lambda *a: 4096)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 7, raising=False)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     monkeypatch.setitem(kernels._q8_ws, (0, 7), ws)
     inside, most, done = [0], [0], []
 
@@ -239,3 +240,37 @@ def test_page_dequant_keeps_its_copy_of_the_ids(monkeypatch):
     kernels.page_dequant(torch.zeros(4, 2, 16, 64).to(E4M3), torch.ones(4, 2),
                          torch.zeros(6, dtype=torch.int32)[::2])
     assert len(copies) == 1
+
+
+def test_capture_on_another_device_takes_the_graphs_memory(monkeypatch):
+    # q on a device that is not the current one, whose stream is being captured: the scratch must not
+    # be the one that eager calls on that stream use
+    current = [0]
+
+    class On:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *a):
+            current[0] = self.before
+
+    kept = kernels.Workspace(torch.device("cpu"))
+    kept.get(1 << 21)
+    real_empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: real_empty(*a, **{**k, "device": "cpu"}))
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == 1)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 7, raising=False)
+    monkeypatch.setattr(kernels, "_check_one_device", lambda *t: torch.device("cuda", 1))
+    monkeypatch.setattr(kernels, "_q8_decode_workspace_bytes", lambda *a: 1 << 21)
+    monkeypatch.setitem(kernels._q8_ws, (1, 7), kept)
+    _build.build()
+    seen = []
+    monkeypatch.setattr(kernels, "_call_on", lambda device, func, *args: seen.append(args))
+    a = _args()
+    kernels.paged_decode_attention_q8(**a, out=torch.zeros_like(a["q"]))
+    assert len(seen) == 1 and kept.buf.data_ptr() not in seen[0]
