@@ -313,15 +313,10 @@ def _check_one_device(*tensors: torch.Tensor | None) -> torch.device:
     return device  # type: ignore[return-value]
 
 
-def _head_rows(t: torch.Tensor) -> bool:
-    """Whether t [n, heads, D] has contiguous heads (a single head's stride means nothing)."""
-    return t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == t.shape[2])
-
-
 def _call_on(device: torch.device, func: str, *args) -> None:
     """_capi.call on the current stream of `device`, with that device current."""
     stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         _capi.call(func, *args, stream)
         return
     with torch.cuda.device(device):
@@ -355,7 +350,12 @@ def rope_append(
     < 0: no K/V row). inv_freq fp32 [R / 2] turns the first R elements of a head
     (rope_frequencies): pairs (j, j + R/2), or (2j, 2j + 1) with `interleaved`; rope_scale
     multiplies cosine and sine. Angles are formed in 64 bits, so far positions keep their
-    precision. Returns q_out [T, Hq, D], which must not overlap the inputs.
+    precision. QK-norm weights are taken in q's dtype, others are rounded to it first, as in
+    decode_prologue. Returns q_out [T, Hq, D], which must not overlap the inputs.
+
+    For one token per request, half layout over the whole head and 16/32-bit pools,
+    decode_prologue does the same in the same time, with the reference's fp32 angles; take
+    rope_append for prompts, far positions, other rotary forms and 8-bit pools.
 
     16/32-bit pools take the rows in the pool dtype, which is q_out's too. Pools of
     torch.float8_e4m3fn need k_scale and v_scale, fp32 [num_pages, Hkv] (q_out then has q's
@@ -388,7 +388,8 @@ def rope_append(
     pool_code = _capi.PI_DTYPE_E4M3 if eight else dtype_code(k_pool.dtype)
     out_dtype = q.dtype if eight else k_pool.dtype
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if not _head_rows(t):
+        # (a single head's stride means nothing)
+        if t.stride(2) != 1 or (t.stride(1) != D and t.shape[1] != 1):
             raise ValueError(f"{name}: heads must be contiguous rows of head_dim elements")
     if positions.dtype != torch.int64 or positions.shape != (T,):
         raise ValueError("positions must be int64 [T]")
@@ -400,7 +401,8 @@ def rope_append(
         raise ValueError("give both QK-norm weights or neither")
     if q_out is None:
         q_out = torch.empty((T, Hq, D), dtype=out_dtype, device=q.device)
-    elif q_out.dtype != out_dtype or tuple(q_out.shape) != (T, Hq, D) or not _head_rows(q_out):
+    elif q_out.dtype != out_dtype or tuple(q_out.shape) != (T, Hq, D) or q_out.stride(2) != 1 \
+            or (q_out.stride(1) != D and Hq != 1):
         raise ValueError(f"q_out must be [T, Hq, D] {out_dtype} with contiguous heads")
     qw = kw = None
     if q_norm_weight is not None:
@@ -686,25 +688,24 @@ def _check_q8_pools(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.T
 
 def _capturing(device: torch.device) -> bool:
     """Whether the current stream of `device`, current or not, is being captured."""
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
 
 
-def _q8_call(device: torch.device, head_dim: int, nbytes: int, workspace: Workspace | None,
-             err: torch.Tensor | None, func: str, *args) -> None:
+def _q8_call(device: torch.device, nbytes: int, lent: bool, workspace: Workspace | None,
+             err: torch.Tensor | None, func: str, args: tuple) -> None:
     """One q8 attention call on the device's current stream, with `nbytes` of scratch: the
     caller's, or one of the stream's own, so that calls on two streams never share it. A call
     may be several launches that hand data over through the scratch, so it is held against
     other threads until all are enqueued. Under graph capture it comes out of the graph's
     memory, zeroed by the graph: no two graphs share it either.
 
-    Scratch for widened pages (nbytes past the decode kernels') grows with the history, so it is
-    not kept: torch's allocator lends it for the call, in powers of two, that a prompt taken in
-    chunks leaves a few blocks behind and not one per chunk. It need not be zeroed."""
+    Scratch for widened pages (`lent`) grows with the history, so it is not kept: torch's
+    allocator lends it for the call, in powers of two, that a prompt taken in chunks leaves a few
+    blocks behind and not one per chunk. It need not be zeroed."""
     if workspace is None:
-        lent = nbytes > _q8_decode_workspace_bytes(device, head_dim)
         capturing = _capturing(device)
         if lent or capturing:
             size = nbytes if capturing else 1 << (nbytes - 1).bit_length()
@@ -722,7 +723,9 @@ def _q8_call(device: torch.device, head_dim: int, nbytes: int, workspace: Worksp
     elif torch.device(workspace.device).index not in (None, device.index):
         raise ValueError(f"the workspace is on {workspace.device}, q on {device}")
     with workspace.lock:
-        buf = workspace.get(nbytes)
+        buf = workspace.buf
+        if buf is None or buf.numel() < nbytes:
+            buf = workspace.get(nbytes)
         _call_on(device, func, *args, buf.data_ptr(), buf.numel(), _err_ptr(err))
 
 
@@ -772,13 +775,14 @@ def paged_decode_attention_q8(
     if ctx_lens.dtype != torch.int32 or ctx_lens.shape != (B,):
         raise ValueError("ctx_lens must be int32 [B]")
     device = _check_one_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, ctx_lens, out, err)
-    if not _head_rows(q) or (B > 1 and q.stride(0) < Hq * D):
+    if q.stride(2) != 1 or (q.stride(1) != D and Hq != 1) or (B > 1 and q.stride(0) < Hq * D):
         q = q.contiguous()
     if block_tables.stride(1) != 1 or ctx_lens.stride(0) != 1:  # (rows may be apart)
         block_tables, ctx_lens = _early_reads(block_tables, ctx_lens)
     if out is None:
         out = torch.empty((B, Hq, D), dtype=q.dtype, device=device)
-    elif out.shape != (B, Hq, D) or out.dtype != q.dtype or not _head_rows(out):
+    elif out.shape != (B, Hq, D) or out.dtype != q.dtype or out.stride(2) != 1 \
+            or (out.stride(1) != D and Hq != 1):
         raise ValueError("out must be [B, Hq, D] with contiguous heads, q's dtype")
     if B == 0:
         return out
@@ -786,11 +790,11 @@ def paged_decode_attention_q8(
         scale = 1.0 / math.sqrt(D)
     row = Hq * D
     _q8_call(
-        device, D, _q8_decode_workspace_bytes(device, D), workspace, err, "pi_paged_decode_attn_q8",
-        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), block_tables.data_ptr(), block_tables.stride(0) if B > 1 else 0,
-        block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv, D, S, P, float(scale), code,
-        q.stride(0) if B > 1 else row, out.stride(0) if B > 1 else row,
+        device, _q8_decode_workspace_bytes(device, D), False, workspace, err, "pi_paged_decode_attn_q8",
+        (out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+         v_scale.data_ptr(), block_tables.data_ptr(), block_tables.stride(0) if B > 1 else 0,
+         block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv, D, S, P, float(scale), code,
+         q.stride(0) if B > 1 else row, out.stride(0) if B > 1 else row),
     )
     return out
 
@@ -817,7 +821,9 @@ def paged_prefill_attention_q8(
     [q_len, Hq, D] in q's dtype (the input's leading batch axis is kept when given). Long chunks
     widen the request's pages once into the workspace and run the tcgen05 prefill on them; short
     ones, and shapes that it does not take, run the 8-bit decode kernels over several rows. Without
-    `workspace` the widened pages are lent by torch's allocator for the call.
+    `workspace` the widened pages are lent by torch's allocator for the call. Widened values and
+    the softmax weights on them are of q's dtype (include/plastic_kv.h states what either path
+    rounds), so outputs of short and long chunks may differ by that.
     """
     P, Hkv, S, D = _check_q8_pools(k_pool, v_pool, k_scale, v_scale)
     batched = q.dim() == 4
@@ -836,7 +842,7 @@ def paged_prefill_attention_q8(
     if kv_len > block_table.numel() * S or kv_len < 0 or q_start < 0 or q_start + n > 2 ** 31 - 1:
         raise ValueError("kv_len must be within the block table's pages, q_start not negative")
     device = _check_one_device(q3, k_pool, v_pool, k_scale, v_scale, block_table, out, err)
-    if not _head_rows(q3) or (n > 1 and q3.stride(0) < Hq * D):
+    if q3.stride(2) != 1 or (q3.stride(1) != D and Hq != 1) or (n > 1 and q3.stride(0) < Hq * D):
         q3 = q3.contiguous()
     if block_table.stride(0) != 1:
         block_table, = _early_reads(block_table)
@@ -844,23 +850,24 @@ def paged_prefill_attention_q8(
         out3 = torch.empty((n, Hq, D), dtype=q3.dtype, device=device)
     else:
         out3 = out[0] if out.dim() == 4 else out
-        if out3.shape != (n, Hq, D) or out3.dtype != q3.dtype or not _head_rows(out3):
+        if out3.shape != (n, Hq, D) or out3.dtype != q3.dtype or out3.stride(2) != 1 \
+                or (out3.stride(1) != D and Hq != 1):
             raise ValueError("out must be [q_len, Hq, D] in q's dtype with contiguous heads")
     if n > 0:
         if scale is None:
             scale = 1.0 / math.sqrt(D)
-        nbytes = _q8_decode_workspace_bytes(device, D)
+        nbytes = kept = _q8_decode_workspace_bytes(device, D)
         if n * Hq > _capi.Q8_FEW_ROWS:  # (fewer rows need the decode scratch only)
             with torch.cuda.device(device):
                 nbytes = int(_capi.load().pi_paged_prefill_attn_q8_workspace_bytes(
                     n, kv_len, Hq, Hkv, D, S, code))
         row = Hq * D
         _q8_call(
-            device, D, nbytes, workspace, err, "pi_paged_prefill_attn_q8",
-            out3.data_ptr(), q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-            k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), block_table.numel(), n,
-            kv_len, q_start, 1 if causal else 0, Hq, Hkv, D, S, P, float(scale), code,
-            q3.stride(0) if n > 1 else row, out3.stride(0) if n > 1 else row,
+            device, nbytes, nbytes > kept, workspace, err, "pi_paged_prefill_attn_q8",
+            (out3.data_ptr(), q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+             k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(), block_table.numel(), n,
+             kv_len, q_start, 1 if causal else 0, Hq, Hkv, D, S, P, float(scale), code,
+             q3.stride(0) if n > 1 else row, out3.stride(0) if n > 1 else row),
         )
     if out is not None:
         return out

@@ -176,7 +176,7 @@ def test_a_call_is_not_split_by_another_thread(monkeypatch, hidden):
     monkeypatch.setattr(kernels, "_q8_decode_workspace_bytes", lambda *a: 4096)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 7, raising=False)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     monkeypatch.setitem(kernels._q8_ws, (0, 7), ws)
     inside, most, done = [0], [0], []
 
@@ -262,7 +262,7 @@ def test_capture_on_another_device_takes_the_graphs_memory(monkeypatch):
     real_empty = torch.empty
     monkeypatch.setattr(torch, "empty", lambda *a, **k: real_empty(*a, **{**k, "device": "cpu"}))
     monkeypatch.setattr(torch.cuda, "device", On)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == 1)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 7, raising=False)
     monkeypatch.setattr(kernels, "_check_one_device", lambda *t: torch.device("cuda", 1))
