@@ -486,8 +486,11 @@ int pi_rope_append(void* q_out, int64_t q_out_stride, void* k_pool, void* v_pool
  *   out[b, hq, :] = softmax(scale * q[b, hq, :] . (sk K)_b[hq / G]^T) (sv V)_b[hq / G]
  * over the first min(ctx_lens[b], max_pages * page_size) tokens of request b; none: zeros.
  * What lies behind a request's last token, in its last page or elsewhere, is not used,
- * whatever bytes it holds. fp32 softmax and accumulation; q and the softmax weights enter the
- * products as sums of e4m3 parts, two for bf16 and three for f16.
+ * whatever bytes it holds. fp32 softmax and accumulation. On the tensor cores K and V are
+ * widened to f16 without loss; q is rounded to f16 at a power-of-two scale of its row (nothing
+ * is lost down to 2^-21 of the row's largest element), and a softmax weight, times its page's V
+ * scale, to f16 relative to the largest of its 32 tokens: by 2^-11 of itself or 2^-33 of that
+ * largest. The plain kernel (below) rounds neither.
  *
  *   q, out         [batch, num_q_heads, head_dim] of `dtype` (f32, bf16, f16), request strides
  *   block_tables   [batch, max_pages] int32, rows bt_stride elements apart (0: one table for all)
@@ -526,7 +529,11 @@ int pi_paged_decode_attn_q8(void* out, const void* q, const void* k_pool, const 
  * not. Any head ratio; q and out of f32, bf16 or f16; head_dim <= 256. Rows that see no key are
  * zero. Many query rows: the pages are widened into `workspace` in q's type (exact in bf16 for
  * power-of-two scales; an f16 value past 65504 becomes 65504) and pi_paged_prefill_attn_tc runs
- * on them; few, or shapes that it does not take: the kernels of pi_paged_decode_attn_q8.
+ * on them, whose softmax weights are of q's type (2^-8 of a weight in bf16); few, or shapes that
+ * it does not take: the kernels of pi_paged_decode_attn_q8. So a request's outputs may differ by
+ * these roundings between a call of few rows and one of many. A NaN in the V row of a key that
+ * the causal mask hides from a query, but that lies in the same tile of keys as one it sees,
+ * makes that query's outputs NaN (a weight of zero times NaN); NaN in hidden K rows does not.
  *   workspace   pi_paged_prefill_attn_q8_workspace_bytes(...) bytes; it begins with the
  *               scratch of pi_paged_decode_attn_q8, whose zeroed part is as there, and so is
  *               the rule for calls that share one. Where these bytes are more than

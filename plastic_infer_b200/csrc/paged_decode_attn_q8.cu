@@ -8,10 +8,12 @@
 // per clock and SM with fresh operands, against 0.30 for the 16-bit m16n8k16 it is put together
 // from. So a unit's values are widened once, in registers, by cvt.rn.f16x2.e4m3x2 (1.2 per clock
 // and SM; every e4m3 value is an f16 value), and both products are f16 MMAs with fp32 sums:
-//   q 2^k in f16: exact for bf16 (down to 2^-22 of the row's largest element, which k brings into
-//   [128, 256)) and for f16;
-//   P in f16, relative to the unit's own maximum and to its larger V scale, times 256: 2^-12 of
-//   each weight, down to 2^-32 of the unit's largest.
+//   q 2^k in f16: exact for bf16 and f16 down to 2^-21 of the row's largest element, which k
+//   brings into [128, 256);
+//   P in f16, relative to the unit's own maximum and to its larger V scale, times 256: half a step is
+//   2^-11 of each weight, or 2^-33 of the unit's largest. A page whose V scale is 2^-k of its
+//   neighbour's in the unit has its weights k bits lower, and loses what falls below.
+// In e4m3 parts (two for bf16, three for f16) both took more MMAs than widening takes conversions.
 //
 // A step of a warp is a unit of 32 tokens (two pages of 16, or one of 32):
 //   S^T[tokens, heads] = K[tokens, D] . Q^T           A = K by ldmatrix, widened
@@ -1014,7 +1016,7 @@ bool fast_shape(int dtype, int requests, int hkv, int64_t passes, int D, int S, 
 template <typename T, int D, int S, int NT, bool kChunk>
 int launch(const Params& p, const void* k_pool, const void* v_pool, cudaStream_t stream) {
   auto kern = decode_q8_kernel<T, D, S, NT, kChunk>;
-  static std::atomic<int> configured[64];  // CTAs per SM + 1, per device
+  static std::atomic<int> configured[64];  // per device: the shared memory limit is set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return PI_ERR_CUDA;
   if (dev < 0 || dev >= 64) return PI_ERR_UNSUPPORTED;
@@ -1025,8 +1027,7 @@ int launch(const Params& p, const void* k_pool, const void* v_pool, cudaStream_t
       return PI_ERR_CUDA;
     configured[dev].store(1, std::memory_order_release);
   }
-  // two CTAs share an SM while the prefix table leaves room for both
-  // two CTAs share an SM while the tables leave room for both
+  // two CTAs share an SM while the prefix tables leave room for both
   const int per_sm = D <= 128 && 2 * (smem + 1024) <= 228 * 1024 ? 2 : 1;
   const uint64_t rows = static_cast<uint64_t>(p.num_pages) * p.hkv * (S * D / 128);
   CUtensorMap tk, tv;

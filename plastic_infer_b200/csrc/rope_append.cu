@@ -31,10 +31,12 @@
 // eight pairs, so a pair never crosses lanes: two 16-byte loads (16-bit types) eight pairs
 // apart in the half layout, adjacent in the interleaved one.
 //
-// Measured on B200 (32 query and 8 KV heads of 128, bf16, QK-norm): 8192 tokens in 54 us, 3.8 TB/s,
-// 0.57 of the measured copy rate; into e4m3 pools 76 us, 0.37 (a block's two barriers and its
-// maximum before anything is written). Two rows' loads in flight per lane were slower (72 us: 80
-// registers instead of 56 leave fewer warps). 64 tokens take 6.4 and 8.4 us in a graph.
+// Measured on B200 (32 query and 8 KV heads of 128, bf16, QK-norm): 8192 tokens in 53 us, 3.8 TB/s,
+// 0.57 of the measured copy rate; into e4m3 pools 75 us, 0.37. The counters name no single limit: an
+// instruction issues in 67 % of the cycles (60 % into e4m3 pools, where 79 registers leave fewer warps),
+// waits on loads and on shared memory make up most of the rest, DRAM is at 36 % (23 %). Two rows' loads
+// in flight per lane were slower (72 us: 80 registers instead of 56 leave fewer warps). 64 tokens
+// take 4.4 and 6.4 us in a graph, the former as decode_prologue.cu does.
 #include <type_traits>
 
 #include <cuda_fp8.h>
