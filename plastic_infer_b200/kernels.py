@@ -700,28 +700,32 @@ def _q8_call(device: torch.device, nbytes: int, lent: bool, workspace: Workspace
     caller's, or one of the stream's own, so that calls on two streams never share it. A call
     may be several launches that hand data over through the scratch, so it is held against
     other threads until all are enqueued. Under graph capture it comes out of the graph's
-    memory, zeroed by the graph: no two graphs share it either.
+    memory, zeroed by the graph: no two graphs share it either. So it does where the caller's
+    workspace is too small yet: the workspace is left as it was.
 
     Scratch for widened pages (`lent`) grows with the history, so it is not kept: torch's
     allocator lends it for the call, in powers of two, that a prompt taken in chunks leaves a few
     blocks behind and not one per chunk. It need not be zeroed."""
-    if workspace is None:
-        capturing = _capturing(device)
-        if lent or capturing:
-            size = nbytes if capturing else 1 << (nbytes - 1).bit_length()
-            buf = torch.empty(size, dtype=torch.uint8, device=device)
-            if not lent:
-                buf[:int(_capi.load().pi_paged_decode_attn_q8_ws_zero_bytes())].zero_()
-            _call_on(device, func, *args, buf.data_ptr(), size, _err_ptr(err))
-            return
+    if workspace is not None and torch.device(workspace.device).index not in (None, device.index):
+        raise ValueError(f"the workspace is on {workspace.device}, q on {device}")
+    lent = lent and workspace is None
+    # (a caller's workspace that would have to grow under capture: what it grew by would be zeroed by
+    # that graph's replays only)
+    capturing = (workspace is None or workspace.buf is None or workspace.buf.numel() < nbytes) \
+        and _capturing(device)
+    if lent or capturing:
+        size = nbytes if capturing else 1 << (nbytes - 1).bit_length()
+        buf = torch.empty(size, dtype=torch.uint8, device=device)
+        if not lent:
+            buf[:int(_capi.load().pi_paged_decode_attn_q8_ws_zero_bytes())].zero_()
+        _call_on(device, func, *args, buf.data_ptr(), size, _err_ptr(err))
+        return
     if workspace is None:
         stream = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
         workspace = _q8_ws.get(stream)
         if workspace is None:
             with _ws_lock:
                 workspace = _q8_ws.setdefault(stream, Workspace(device))
-    elif torch.device(workspace.device).index not in (None, device.index):
-        raise ValueError(f"the workspace is on {workspace.device}, q on {device}")
     with workspace.lock:
         buf = workspace.buf
         if buf is None or buf.numel() < nbytes:

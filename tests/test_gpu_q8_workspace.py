@@ -140,3 +140,30 @@ def test_lent_scratch_need_not_be_zeroed():
         dirty = torch.full((64 << 20,), 0xA5, dtype=torch.uint8, device=DEV)
         del dirty
         check(prefill(q, c, n, n - 420)[rows], ref, tol)
+
+
+@pytest.mark.parametrize("lens", [[3000], [700] * 40], ids=["merge launch", "last arriver"])
+def test_two_graphs_over_a_cold_workspace(lens):
+    # neither graph has grown it for the other, nor for an eager call before any replay
+    c = on_gpu(cache(lens, 8, 128, 16, seed=90))
+    q = queries(len(lens), 32, 128, torch.bfloat16, 90)
+    want = decode(q, c).clone()
+    ws = kernels.Workspace(DEV)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = decode(q, c, workspace=ws)
+        graphs.append((g, out))
+    assert ws.buf is None
+    assert torch.equal(decode(q, c, workspace=ws), want)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):  # the second first, then both at once
+        for s, (g, _out) in zip(streams, reversed(graphs)):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for _g, out in graphs:
+        assert torch.equal(out, want)
+    assert torch.equal(decode(q, c, workspace=ws), want)

@@ -274,3 +274,33 @@ def test_capture_on_another_device_takes_the_graphs_memory(monkeypatch):
     a = _args()
     kernels.paged_decode_attention_q8(**a, out=torch.zeros_like(a["q"]))
     assert len(seen) == 1 and kept.buf.data_ptr() not in seen[0]
+
+
+@pytest.mark.parametrize("warm", [False, True])
+def test_workspace_under_capture(monkeypatch, warm):
+    # a workspace that would have to grow under capture is left alone: memory that only one graph's
+    # replays zero must not be what another graph or an eager call finds there
+    zero = []
+
+    class Lib:
+        def pi_paged_decode_attn_q8_ws_zero_bytes(self):
+            zero.append(True)
+            return 1024
+
+    ws = kernels.Workspace(torch.device("cpu"))
+    if warm:
+        ws.get(1 << 21)
+    before = ws.buf
+    real_empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: real_empty(*a, **{**k, "device": "cpu"}))
+    monkeypatch.setattr(_capi, "load", lambda: Lib())
+    monkeypatch.setattr(kernels, "_check_one_device", lambda *t: torch.device("cuda", 0))
+    monkeypatch.setattr(kernels, "_q8_decode_workspace_bytes", lambda *a: 1 << 21)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    seen = []
+    monkeypatch.setattr(kernels, "_call_on", lambda device, func, *args: seen.append(args))
+    a = _args()
+    kernels.paged_decode_attention_q8(**a, out=torch.zeros_like(a["q"]), workspace=ws)
+    assert ws.buf is before and len(seen) == 1
+    assert (before is not None and before.data_ptr() in seen[0]) == warm and bool(zero) != warm
