@@ -506,7 +506,8 @@ class Workspace:
         with self.lock:
             buf = self.buf
             if buf is None or buf.numel() < nbytes:
-                n = max(nbytes, 1 << 20)
+                # (twice as large at least: a history that grows call by call is not a buffer a call)
+                n = max(nbytes, 1 << 20, 0 if buf is None else 2 * buf.numel())
                 self.buf = buf = torch.zeros(n, dtype=torch.uint8, device=self.device)
             return buf
 

@@ -304,3 +304,12 @@ def test_workspace_under_capture(monkeypatch, warm):
     kernels.paged_decode_attention_q8(**a, out=torch.zeros_like(a["q"]), workspace=ws)
     assert ws.buf is before and len(seen) == 1
     assert (before is not None and before.data_ptr() in seen[0]) == warm and bool(zero) != warm
+
+
+def test_workspace_grows_in_few_steps():
+    ws = kernels.Workspace(torch.device("cpu"))
+    buffers = set()
+    for i in range(1, 41):
+        assert ws.get(i << 20).numel() >= i << 20
+        buffers.add(ws.buf.numel())
+    assert len(buffers) <= 7 and max(buffers) < 2 * (40 << 20)
