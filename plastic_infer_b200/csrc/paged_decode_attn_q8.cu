@@ -13,7 +13,8 @@
 //   P in f16, relative to the unit's own maximum and to its larger V scale, times 256: half a step is
 //   2^-11 of each weight, or 2^-33 of the unit's largest. A page whose V scale is 2^-k of its
 //   neighbour's in the unit has its weights k bits lower, and loses what falls below.
-// In e4m3 parts (two for bf16, three for f16) both took more MMAs than widening takes conversions.
+// (q and P in e4m3 parts, two for bf16 and three for f16, with K and V as they are: 112.6 us for the 64
+// requests below.)
 //
 // A step of a warp is a unit of 32 tokens (two pages of 16, or one of 32):
 //   S^T[tokens, heads] = K[tokens, D] . Q^T           A = K by ldmatrix, widened
